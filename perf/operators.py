@@ -233,7 +233,7 @@ def _prepare_adamw(case, r):
     else:
         half = torch.full((blocks, BLOCK), 1 << 15, dtype=torch.int32, device="cuda")
         s["m"], s["me"] = _encode(m, half)
-        s["v"], s["ve"] = _encode(root, half)
+        s["v"], s["ve"] = _encode(root, half, True)
     return s
 
 
@@ -446,17 +446,22 @@ def _powers(case):
     return F32(F32(B1) ** case["step"]), F32(F32(B2) ** case["step"])
 
 
-def _encode(x, rnd):
+def _encode(x, rnd, square=False):
     """Blocks of values -> e4m3 codes (exponent 1 .. 15 of bias 7, three mantissa bits; sign on top) of
-    x / 2^(E - 127) and the blocks' E: the largest value lands in [2^7, 2^8).  A value goes up or down by
-    its 16 bits of rnd, in proportion to its distance from either."""
-    bits = x.abs().view(torch.int32)
-    E = ((bits.amax(1) >> 23) - 7).clamp(min=1)
+    x / 2^(E - 127) and the blocks' E: the largest value lands in [2^7, 2^8).  A value between two codes goes
+    up where its 16 bits of rnd, as a fraction, are below its share of the gap; square: the square's share
+    of the gap between the codes' squares."""
+    E = ((x.abs().view(torch.int32).amax(1) >> 23) - 7).clamp(min=1)
     y = x.abs() * ((254 - E) << 23).view(torch.float32)[:, None]
-    normal = ((y.view(torch.int32) + (rnd << 4)) >> 20) - (120 << 3)
-    small = torch.floor(y * 512.0 + rnd.float() * 2.0**-16).to(torch.int32)
-    code = torch.where(y >= 2.0**-6, normal, small) | torch.where(x < 0, 128, 0)
-    return code.to(torch.uint8), E.to(torch.uint8)
+    bits, normal = y.view(torch.int32), y >= 2.0**-6
+    small = torch.floor(y * 512.0)
+    low = torch.where(normal, (bits & -(1 << 20)).view(torch.float32), small * 2.0**-9)
+    high = torch.where(normal, ((bits & -(1 << 20)) + (1 << 20)).view(torch.float32), low + 2.0**-9)
+    gap, rest = high - low, y - low
+    if square:
+        gap, rest = gap * (high + low), rest * (y + low)
+    code = torch.where(normal, (bits >> 20) - (120 << 3), small.to(torch.int32)) + (rnd.float() * 2.0**-16 * gap < rest)
+    return (code | torch.where(x < 0, 128, 0)).to(torch.uint8), E.to(torch.uint8)
 
 
 def _decode(code, E):
@@ -499,7 +504,7 @@ def _adamw_plain(s):
     code, E = _encode(m, (rnd & 0xFFFF).to(torch.int32))
     s["m"].copy_(code)
     s["me"].copy_(E)
-    code, E = _encode(root, (rnd >> 16).to(torch.int32))
+    code, E = _encode(root, (rnd >> 16).to(torch.int32), True)
     s["v"].copy_(torch.where(root > 0, code.clamp(min=1), code))
     s["ve"].copy_(E)
     return _adamw_states(s)
@@ -536,13 +541,14 @@ def _adamw_exact(case, seed):
         v = torch.where(ex > 0, (8 + ma).to(d) * torch.pow(2.0, (ex - 10).to(d)), ma.to(d) * 2.0**-9)
         return torch.where(x > 127, -v, v) * torch.pow(2.0, e.to(d) - 127)[:, None]
 
-    def stored(x, rnd, least):
+    def stored(x, rnd, power):
         ex = torch.floor(torch.log2(x.abs().amax(1, keepdim=True))) - 7  # the block's unit, a power of two
         ex = torch.where(torch.isfinite(ex), ex, -126.0).clamp(min=-126)
         y = x.abs() * torch.pow(2.0, -ex)
         step = torch.pow(2.0, torch.floor(torch.log2(y.clamp(min=2.0**-6))) - 3)
-        q = torch.floor(y / step + rnd.to(d) / 65536) * step
-        return torch.sign(x) * torch.where((x != 0) & least, q.clamp(min=2.0**-9), q)
+        low = torch.floor(y / step) * step
+        share = (y**power - low**power) / ((low + step) ** power - low**power)
+        return torch.sign(x) * torch.where((rnd.to(d) / 65536 < share), low + step, low)
 
     g = s["g"].double()
     m, v = (s["m"].double(), s["v"].double()) if case["bits"] == 32 else (value(s["m"], s["me"]), value(s["v"], s["ve"]) ** 2)
@@ -553,8 +559,8 @@ def _adamw_exact(case, seed):
     if case["bits"] == 32:
         return {"p": p, "m": m, "v": v}
     rnd = _random(s)
-    no, yes = torch.tensor(False, device="cuda"), torch.tensor(True, device="cuda")
-    return {"p": p, "m": stored(m, rnd & 0xFFFF, no), "v": stored(torch.sqrt(v), rnd >> 16, yes), "me": None, "ve": None}
+    root = stored(torch.sqrt(v), rnd >> 16, 2)
+    return {"p": p, "m": stored(m, rnd & 0xFFFF, 1), "v": torch.where(v > 0, root.clamp(min=2.0**-9), root), "me": None, "ve": None}
 
 
 # ------------------------------------------------------------------------------------------------
