@@ -62,6 +62,18 @@ class NanoLLMWeightsC(ctypes.Structure):
                 ("lnf_gamma", _f32p), ("lnf_beta", _f32p), ("lm_head", _f32p)]
 
 
+class PackedAttention(ctypes.Structure):
+    """fmlh_packed_attention: sizes, strides (in floats) and device offsets of packed sequences."""
+
+    _fields_ = [("n_seq", _u32), ("q_rows", _u32), ("k_rows", _u32), ("n_head", _u32), ("n_kv_head", _u32),
+                ("head_dim", _u32), ("scale", ctypes.c_float), ("q_off", _vp), ("k_off", _vp), ("k_len", _vp),
+                ("q_rs", _sz), ("o_rs", _sz), ("k_rs", _sz), ("v_rs", _sz), ("k_hs", _sz), ("v_hs", _sz)]
+
+
+class AdamWTensor(ctypes.Structure):
+    _fields_ = [("param", _vp), ("grad", _vp), ("m", _vp), ("v", _vp), ("m_exp", _vp), ("v_exp", _vp), ("n", _sz)]
+
+
 _SIGS = {
     "fmlh_init": [ctypes.c_int],
     "fmlh_shutdown": [],
@@ -108,6 +120,13 @@ _SIGS = {
     "fmlh_merge_qkv": [_vp] * 4 + [_u32] * 3,
     "fmlh_attention_softmax_heads": [ctypes.POINTER(_vp), _sz, _vp, _vp, _vp, _u32, _u32],
     "fmlh_attention_softmax_backward_heads": [_vp, ctypes.POINTER(_vp), _vp, _vp, _u32, _u32],
+    "fmlh_attention_packed_workspace": [ctypes.POINTER(PackedAttention), ctypes.c_int, ctypes.POINTER(_sz)],
+    "fmlh_attention_packed": [ctypes.POINTER(PackedAttention)] + [_vp] * 6 + [_sz],
+    "fmlh_attention_packed_backward": [ctypes.POINTER(PackedAttention)] + [_vp] * 10 + [_sz],
+    "fmlh_preference_logits": [_vp] * 8 + [_u32] * 3 + [ctypes.c_float] * 2,
+    "fmlh_sequence_logprobs": [_vp] * 5 + [_u32] * 3,
+    "fmlh_preference_workspace": [_u32, _u32, ctypes.POINTER(_sz)],
+    "fmlh_adamw_update_multi": [ctypes.POINTER(AdamWTensor), _u32, ctypes.c_int] + [ctypes.c_float] * 7 + [ctypes.c_uint64],
     "fmlh_nanollm_create": [ctypes.POINTER(NanoLLMConfig), ctypes.POINTER(NanoLLMWeightsC),
                             ctypes.c_int, ctypes.POINTER(_vp)],
     "fmlh_nanollm_destroy": [_vp],
@@ -396,6 +415,55 @@ def dropout_mask(mask, n, uniforms, count, start, prob):
     """DropoutLayer::UpdateMask's draws for 0 < prob < 1 (DropoutLayer.h:97-123) from a device
     copy of RandomUtils' uniform buffer, starting at draw `start`."""
     call("fmlh_dropout_mask", mask, n, uniforms, count, start, prob)
+
+
+# ---- preference tuning and grouped heads ---------------------------------------------------
+
+def attention_packed_workspace(shape: PackedAttention, backward: bool = False) -> int:
+    """Floats of device workspace a forward or backward call of this shape needs."""
+    n = _sz()
+    call("fmlh_attention_packed_workspace", ctypes.byref(shape), 1 if backward else 0, ctypes.byref(n))
+    return n.value
+
+
+def attention_packed(shape, out, lse, q, k, v, ws=0, ws_floats=0):
+    """Causal attention of packed sequences, grouped heads; lse may be 0 (None)."""
+    call("fmlh_attention_packed", ctypes.byref(shape), out, lse or None, q, k, v, ws or None, ws_floats)
+
+
+def attention_packed_backward(shape, dq, dk, dv, dout, out, lse, q, k, v, ws=0, ws_floats=0):
+    """Gradients of attention_packed from dout; out and lse as the forward call left them."""
+    call("fmlh_attention_packed_backward", ctypes.byref(shape), dq, dk, dv, dout, out, lse, q, k, v, ws or None, ws_floats)
+
+
+def preference_workspace(rows, n_seq) -> int:
+    """Floats of device workspace preference_logits (n_seq = 2 pairs) and sequence_logprobs need."""
+    n = _sz()
+    call("fmlh_preference_workspace", rows, n_seq, ctypes.byref(n))
+    return n.value
+
+
+def preference_logits(grad, loss, logp, ws, target, logits, off, ref_logp, vocab, rows, pairs, beta=0.1, smoothing=0.0):
+    """Preference loss (paired log ratios) and its descent direction; grad, loss, logp may be 0 (None)."""
+    call("fmlh_preference_logits", grad or None, loss or None, logp or None, ws, target, logits, off, ref_logp, vocab, rows,
+         pairs, beta, smoothing)
+
+
+def sequence_logprobs(logp, ws, target, logits, off, vocab, rows, n_seq):
+    """Sums of log softmax(logits)[target] over packed sequences."""
+    call("fmlh_sequence_logprobs", logp, ws, target, logits, off, vocab, rows, n_seq)
+
+
+def adamw_tensors(tensors):
+    """The list adamw_update_multi takes, from (param, grad, m, v, n) or, for 8-bit states,
+    (param, grad, m, v, n, m_exp, v_exp) device addresses; it can be kept from step to step."""
+    return (AdamWTensor * len(tensors))(*(AdamWTensor(*t[:4], *(t[5:] or (None, None)), t[4]) for t in tensors))
+
+
+def adamw_update_multi(tensors, state_bits, lr, beta1, beta2, beta1_pow_t, beta2_pow_t, eps, wd, seed=0):
+    """adamw_update over many tensors (adamw_tensors), states in 32 or 8 bits."""
+    call("fmlh_adamw_update_multi", tensors, len(tensors), state_bits, lr, beta1, beta2, beta1_pow_t, beta2_pow_t, eps, wd,
+         seed)
 
 
 _probe_lib = None

@@ -256,6 +256,95 @@ int fmlh_sum_columns(float* out, const float* in, uint32_t rows, uint32_t cols);
 int fmlh_dropout_mask(float* mask, uint64_t n, const float* uniforms, uint64_t count, uint64_t start,
                       float prob);
 
+/* ---- preference tuning and grouped heads (no counterparts in the reference) ------------ */
+
+/* Causal attention of packed sequences, n_head query heads on n_kv_head key heads (head h reads key
+ * head h / (n_head / n_kv_head)).  Query i of a sequence of ql queries and kl keys sees its keys
+ * j <= i + kl - ql: both ends meet, so ql = kl is a whole prompt, ql = 1 a single token over a cache
+ * and what lies between a chunk of a prompt; queries before the first key see none.
+ *   s = scale q . k, p = softmax over the seen keys, out = sum p v, lse = log sum exp(s)
+ * A query that sees no key gets out = 0, lse = -infinity and passes no gradient.
+ *
+ * Sequence s has rows q_off[s] .. q_off[s + 1] - 1 of q, out, dout and dq, and its keys start at row
+ * k_off[s] of k, v, dk and dv: k_len[s] of them, at most up to row k_off[s + 1] (k_len NULL: all up to
+ * there).  The three arrays are device memory, read when the work runs, so that a captured call
+ * follows their contents; offsets must not fall.  Rows that no sequence holds are left as they are.
+ * Element d of head h in row r: q[r q_rs + h head_dim + d], out[r o_rs + h head_dim + d] (dq and dout
+ * likewise), k[r k_rs + h k_hs + d], v[r v_rs + h v_hs + d] (dk and dv likewise).  So the rows of a
+ * QKV product are q, k = q + n_head head_dim, v = k + n_kv_head head_dim with q_rs = k_rs = v_rs its width
+ * and k_hs = v_hs = head_dim; the engine's caches [sequence][head][block_size][head_dim] are k_rs =
+ * head_dim, k_hs = block_size head_dim, k_off[s] = s n_kv_head block_size.
+ * head_dim 1 .. 128, any strides and alignment (16-byte aligned rows and heads are faster). */
+typedef struct fmlh_packed_attention {
+    uint32_t n_seq;
+    uint32_t q_rows, k_rows; /* rows that exist; offsets beyond them are cut */
+    uint32_t n_head, n_kv_head, head_dim;
+    float scale; /* usually 1 / sqrt(head_dim) */
+    const int32_t* q_off; /* n_seq + 1 */
+    const int32_t* k_off; /* n_seq + 1 */
+    const int32_t* k_len; /* n_seq, or NULL */
+    size_t q_rs, o_rs, k_rs, v_rs; /* row strides, in floats */
+    size_t k_hs, v_hs;             /* head strides of k and v, in floats */
+} fmlh_packed_attention;
+
+/* Floats of device workspace that a forward (backward = 0) or backward call of this shape needs; 0:
+ * none.  It depends on the sizes alone, not on the offsets' contents.  A workspace serves one call
+ * at a time: calls and captured graphs that may run at once need one each. */
+int fmlh_attention_packed_workspace(const fmlh_packed_attention* shape, int backward, size_t* floats);
+
+/* lse (n_head x q_rows) may be NULL where no backward pass follows.  out must not overlap the inputs. */
+int fmlh_attention_packed(const fmlh_packed_attention* shape, float* out, float* lse, const float* q,
+                          const float* k, const float* v, float* ws, size_t ws_floats);
+
+/* Gradients of sum(out dout): dq, dk and dv are written, not added to; a key head's gradients are the
+ * sums over its query heads, in a fixed order.  out and lse are the forward call's.  Sequences must
+ * not share keys.  No gradient may overlap another or an input. */
+int fmlh_attention_packed_backward(const fmlh_packed_attention* shape, float* dq, float* dk, float* dv,
+                                   const float* dout, const float* out, const float* lse, const float* q,
+                                   const float* k, const float* v, float* ws, size_t ws_floats);
+
+/* Preference loss on the logits (rows x vocab) of packed pairs: sequence s has rows off[s] ..
+ * off[s + 1] - 1 (device, 2 pairs + 1 offsets that do not fall), 2p the chosen and 2p + 1 the rejected one
+ * of pair p.  target[row] is the row's id, truncated; rows whose id is outside [0, vocab) (-1) do not
+ * count, as in fmlh_cce_logits.  With lp_s the sum of a sequence's log softmax(logits)[target] and
+ * ref_logp (device, 2 pairs) the same of the reference model,
+ *   x_p = beta ((lp_2p - ref_2p) - (lp_2p+1 - ref_2p+1)),
+ *   loss = mean over p of (1 - smoothing) softplus(-x_p) + smoothing softplus(x_p).
+ * grad (NULL: skip) is the descent direction -dloss/dlogits, as fmlh_cce_logits gives it and
+ * fmlh_adamw_update adds it; rows that no sequence holds are left as they are.  grad may be logits.
+ * loss (NULL: skip) is one float, logp (NULL: skip) 2 pairs.  ws: fmlh_preference_workspace floats,
+ * 8-byte aligned, for one call at a time.  Log-probabilities are summed in 64 bits. */
+int fmlh_preference_logits(float* grad, float* loss, float* logp, float* ws, const float* target,
+                           const float* logits, const int32_t* off, const float* ref_logp, uint32_t vocab,
+                           uint32_t rows, uint32_t pairs, float beta, float smoothing);
+/* logp[s] alone, of n_seq sequences (n_seq + 1 offsets): the reference model's part. */
+int fmlh_sequence_logprobs(float* logp, float* ws, const float* target, const float* logits,
+                           const int32_t* off, uint32_t vocab, uint32_t rows, uint32_t n_seq);
+/* Floats of device workspace either needs (n_seq = 2 pairs). */
+int fmlh_preference_workspace(uint32_t rows, uint32_t n_seq, size_t* floats);
+
+/* fmlh_adamw_update over many tensors at once (a launch per 64 of them).  state_bits 32: m and v are
+ * n floats, and the results are fmlh_adamw_update's bit for bit.  state_bits 8: m and v are n bytes,
+ * e4m3 codes of m and of sqrt(v), and m_exp and v_exp a byte E per 256 consecutive elements; a code c of
+ * such a block stands for c 2^(E - 127).  All zero bytes are states of zero.  The update itself takes
+ * the new m and v before they are rounded; they are rounded up or down at random, so that m and v
+ * are kept on average, by a hash of seed, the tensor's place in the list and the element: pass
+ * another seed every step (equal seeds give equal results).  A value that is not finite is
+ * kept as NaN.  The list is host memory and is read before the call returns; no two of its
+ * buffers may share memory (two gradients may). */
+typedef struct fmlh_adamw_tensor {
+    float* param;
+    const float* grad;
+    void* m;
+    void* v;
+    uint8_t* m_exp; /* 8-bit states only */
+    uint8_t* v_exp;
+    size_t n;
+} fmlh_adamw_tensor;
+int fmlh_adamw_update_multi(const fmlh_adamw_tensor* tensors, uint32_t count, int state_bits, float lr,
+                            float beta1, float beta2, float beta1_pow_t, float beta2_pow_t, float eps,
+                            float weight_decay, uint64_t seed);
+
 /* ---- NanoLLM token loop ------------------------------------------------------------- */
 
 typedef struct fmlh_nanollm fmlh_nanollm;
