@@ -8,6 +8,7 @@ namespace fmlh {
 struct PackedAttn {
     uint32_t n_seq, q_rows, k_rows;
     int group;     // query heads per key head
+    uint32_t n_kv; // key heads
     int head_dim;
     float scale;
     int vec;       // every row and head 16-byte aligned, head_dim a multiple of 4

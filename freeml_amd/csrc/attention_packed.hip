@@ -17,98 +17,13 @@
 // Masked scores are replaced before they are used, but 0 * v of a masked infinite or NaN v would
 // still reach a sum on the matrix cores: tiles that hold a masked pair and a value that is not
 // finite are multiplied element by element instead.
-#include "attention_packed.h"
-#include "bf16_split.h"
+#include "attention_packed_device.h"
 
 #include <algorithm>
 
 namespace fmlh {
 
 namespace {
-
-constexpr int kRowsPerWave = 32;
-constexpr int kRowsPerWG = 4 * kRowsPerWave;
-constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-
-__device__ __forceinline__ uint32_t clamp_row(int32_t v, uint32_t rows) {
-    return v < 0 ? 0u : min((uint32_t)v, rows);
-}
-
-// A sequence's rows: offsets outside [0, rows] or falling are cut to what lies inside.
-struct Span {
-    uint32_t q0, ql, k0, kl;
-};
-
-__device__ __forceinline__ Span load_span(const PackedAttn& a, uint32_t s) {
-    Span p;
-    p.q0 = clamp_row(a.q_off[s], a.q_rows);
-    const uint32_t q1 = clamp_row(a.q_off[s + 1], a.q_rows);
-    p.ql = q1 > p.q0 ? q1 - p.q0 : 0u;
-    p.k0 = clamp_row(a.k_off[s], a.k_rows);
-    const uint32_t k1 = clamp_row(a.k_off[s + 1], a.k_rows);
-    p.kl = k1 > p.k0 ? k1 - p.k0 : 0u;
-    if (a.k_len) p.kl = min(p.kl, (uint32_t)max(a.k_len[s], 0));
-    return p;
-}
-
-// The sequence that tile `t` of the launch falls to, where sequence s has ceil(count_s / per) tiles
-// (count: its keys, or its rows of all heads of a group): every wave scans the offsets, 64
-// sequences at a time.  Returns false for tiles behind the last sequence (the grid holds
-// sum / per + n_seq tiles, never fewer than there are).
-template <bool KEYS>
-__device__ __forceinline__ bool find_tile(const PackedAttn& a, uint32_t per, uint32_t t, Span* span, uint32_t* tile,
-                                          uint32_t* tiles) {
-    const uint32_t lane = threadIdx.x & 63;
-    uint32_t before = 0;
-    for (uint32_t base = 0; base < a.n_seq; base += 64) {
-        const uint32_t s = base + lane;
-        uint32_t n = 0;
-        if (s < a.n_seq) {
-            const Span p = load_span(a, s);
-            n = (uint32_t)(((uint64_t)(KEYS ? p.kl : p.ql) * (KEYS ? 1u : a.group) + per - 1) / per);
-        }
-        uint32_t upto = n;  // inclusive scan
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const uint32_t o = __shfl_up(upto, d);
-            if (lane >= (uint32_t)d) upto += o;
-        }
-        const uint64_t hit = __ballot(before + upto > t);
-        if (hit) {
-            const int l = __builtin_ctzll(hit);
-            const uint32_t first = before + __shfl(upto - n, l);
-            *tiles = __shfl(n, l);
-            *tile = t - first;
-            *span = load_span(a, base + l);
-            return true;
-        }
-        before += __shfl(upto, 63);
-    }
-    return false;
-}
-
-// Dims 4 u .. 4 u + 3 of a row, zeros past head_dim.
-__device__ __forceinline__ floatx4 load4(const float* row, int d, int dim, bool vec) {
-    floatx4 v = {0.f, 0.f, 0.f, 0.f};
-    if (vec) {
-        if (d < dim) v = *reinterpret_cast<const floatx4*>(row + d);
-    } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (d + e < dim) v[e] = row[d + e];
-    }
-    return v;
-}
-
-__device__ __forceinline__ void store4(float* row, int d, int dim, bool vec, floatx4 v) {
-    if (vec) {
-        if (d < dim) *reinterpret_cast<floatx4*>(row + d) = v;
-    } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (d + e < dim) row[d + e] = v[e];
-    }
-}
 
 // NaN where a value is infinite or NaN, else 0.
 __device__ __forceinline__ float not_finite(floatx4 v) { return (v[0] + v[1] + v[2] + v[3]) * 0.f; }
@@ -131,13 +46,10 @@ __device__ __forceinline__ float stage_rows(float* lds, const float* base, size_
     return bad;
 }
 
-// Register r of a lane's 32 x 32 accumulator is row 8 (r / 4) + 4 h + r % 4 of it.
-__device__ __forceinline__ int acc_row(int r, int h) { return 8 * (r >> 2) + 4 * h + (r & 3); }
-
 // S (32 x 32) = A B^T over DP dims: A's rows from LDS (row stride LD), B's row of lane column c in
 // registers (dims h DP / 2 ..).  The matrix core's two k of a step are dims u and DP / 2 + u.
 template <int DP, int LD>
-__device__ __forceinline__ floatx16 rows_product(const float* lds_rows, const float (&b)[DP / 2], int h, int c) {
+__device__ __forceinline__ floatx16 lds_rows_product(const float* lds_rows, const float (&b)[DP / 2], int h, int c) {
     floatx16 s;
 #pragma unroll
     for (int r = 0; r < 16; ++r) s[r] = 0.f;
@@ -162,25 +74,213 @@ __device__ __forceinline__ void add_product(floatx16 (&acc)[DP / 32], const floa
     }
 }
 
-// The same element by element, over the pairs `seen` names only (bit r of lane (h, c): row
-// acc_row(r, h), column c).  Rolled up: it runs for tiles that are rare.
-template <int DP, int LD>
-__device__ __forceinline__ void add_seen(floatx16 (&acc)[DP / 32], const float* lds_rows, const floatx16& w, uint32_t seen, int h,
-                                         int c) {
-#pragma unroll 1
-    for (int n = 0; n < 32; ++n) {
-        const int r = n >> 1, from = c + 32 * (n & 1);
-        float mine = 0.f;
+// ---- few rows over many keys -------------------------------------------------------------------
+
+// Single tokens over a cache: with RT rows (the heads of a group, a few queries) the keys' and values'
+// bytes are the work.  A work-group takes a tile of RT rows of one (sequence, key head) and one of
+// the ranges its keys are cut into; LPK lanes hold a key (NF float4 each), 64 / LPK keys per
+// wave and step, kUnroll steps in flight.  Every lane group keeps its own maximum, sum and output
+// over its keys; they are joined over the wave and the work-group once, at the end.
+
+// A tile with one range writes its rows, otherwise their (maximum, sum, output) go to the workspace
+// and are joined by attn_packed_join_kernel in range order.
+// Sum over the LPK lanes of a key (4, 8 or 16, inside a DPP row): every lane holds it afterwards.
+template <int LPK>
+__device__ __forceinline__ float key_sum(float x) {
+    x += dpp_move<0xB1, 0xf>(0.f, x);  // quad_perm [1, 0, 3, 2]
+    x += dpp_move<0x4E, 0xf>(0.f, x);  // quad_perm [2, 3, 0, 1]
+    if (LPK >= 8) x += dpp_move<0x141, 0xf>(0.f, x);   // row_half_mirror
+    if (LPK >= 16) x += dpp_move<0x140, 0xf>(0.f, x);  // row_mirror
+    return x;
+}
+
+template <int LPK, int NF, int RT>
+__global__ __launch_bounds__(256) void attn_packed_few_kernel(PackedAttn a, float* __restrict__ out, float* __restrict__ lse,
+                                                              const float* __restrict__ q, const float* __restrict__ k,
+                                                              const float* __restrict__ v, float* __restrict__ ws, uint32_t budget) {
+    constexpr int KPW = 64 / LPK, UN = RT * NF >= 8 ? 2 : 4, STEP = 4 * KPW * UN, W = 4 * LPK * NF;
+    __shared__ float join_ml[4][RT][2];
+    __shared__ __attribute__((aligned(16))) float join_o[4][RT][W];
+    Work w;
+    if (!find_work<false, false>(a, RT, budget, blockIdx.x, &w)) return;
+    const RowTile tl = row_tile(a, w, RT);
+    if (w.range >= tl.ranges) return;
+    const Span sp = w.sp;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sub = lane % LPK, slot = wave * KPW + lane / LPK;
+    const int dim = a.head_dim, group = a.group, kv = blockIdx.y;
+    const int rows = tl.rows, rho0 = tl.rho0, shift = tl.shift, k_begin = tl.k_begin, k_end = tl.k_end;
+    const float* kb = k + (size_t)sp.k0 * a.k_rs + (size_t)kv * a.k_hs;
+    const float* vb = v + (size_t)sp.k0 * a.v_rs + (size_t)kv * a.v_hs;
+    const float factor = a.scale * kLog2e;
+
+    floatx4 qr[RT][NF], o[RT][NF];
+    float m[RT], l[RT];
+    int limit[RT];
 #pragma unroll
-        for (int t = 0; t < 16; ++t) mine = t == r ? w[t] : mine;
-        const float p = __shfl(mine, from);
-        const bool on = (__shfl((int)seen, from) >> r) & 1;
-        const float* x = lds_rows + acc_row(r, n & 1) * LD;
+    for (int t = 0; t < RT; ++t) {
+        const int rho = min(rho0 + t, rows - 1);
+        const float* row = q + (size_t)(sp.q0 + rho / group) * a.q_rs + (size_t)(kv * group + rho % group) * dim;
 #pragma unroll
-        for (int i = 0; i < DP / 32; ++i)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) acc[i][e] += on ? p * x[32 * i + acc_row(e, h)] : 0.f;
+        for (int f = 0; f < NF; ++f) {
+            qr[t][f] = load4(row, 4 * (sub + LPK * f), dim, a.vec);
+            o[t][f] = floatx4{0.f, 0.f, 0.f, 0.f};
+        }
+        m[t] = -INFINITY;
+        l[t] = 0.f;
+        limit[t] = rho / group + shift;
     }
+    for (int j0 = k_begin; j0 < k_end; j0 += STEP) {
+        floatx4 kx[UN][NF], vx[UN][NF];
+#pragma unroll
+        for (int u = 0; u < UN; ++u) {
+            const size_t j = min(j0 + u * 4 * KPW + slot, k_end - 1);
+#pragma unroll
+            for (int f = 0; f < NF; ++f) kx[u][f] = load4(kb + j * a.k_rs, 4 * (sub + LPK * f), dim, a.vec);
+#pragma unroll
+            for (int f = 0; f < NF; ++f) vx[u][f] = load4(vb + j * a.v_rs, 4 * (sub + LPK * f), dim, a.vec);
+        }
+        const bool all = j0 + STEP <= min(k_end, rho0 / group + shift + 1);  // every row sees every key of the step
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+            float s[UN], top = m[t];
+#pragma unroll
+            for (int u = 0; u < UN; ++u) {
+                float d = 0.f;
+#pragma unroll
+                for (int f = 0; f < NF; ++f)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) d += qr[t][f][e] * kx[u][f][e];
+                s[u] = key_sum<LPK>(d) * factor;
+                if (!all && j0 + u * 4 * KPW + slot > min(limit[t], k_end - 1)) s[u] = -INFINITY;
+                top = fmaxf(top, s[u]);
+            }
+            const float base = top == -INFINITY ? 0.f : top;
+            const float corr = exp2f(m[t] - base);
+            m[t] = top;
+            l[t] *= corr;
+#pragma unroll
+            for (int f = 0; f < NF; ++f) o[t][f] *= corr;
+#pragma unroll
+            for (int u = 0; u < UN; ++u) {
+                const float p = exp2f(s[u] - base);
+                l[t] += p;
+                if (all) {
+#pragma unroll
+                    for (int f = 0; f < NF; ++f) o[t][f] += p * vx[u][f];
+                } else if (j0 + u * 4 * KPW + slot <= min(limit[t], k_end - 1)) {  // 0 * v of a masked v that is not finite
+#pragma unroll
+                    for (int f = 0; f < NF; ++f) o[t][f] += p * vx[u][f];
+                }
+            }
+        }
+    }
+    // Join the lane groups of the wave, then the waves.
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+        float top = m[t];
+#pragma unroll
+        for (int d = LPK; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
+        const float corr = exp2f(m[t] - (top == -INFINITY ? 0.f : top));
+        float sum = l[t] * corr;
+#pragma unroll
+        for (int f = 0; f < NF; ++f) o[t][f] *= corr;
+#pragma unroll
+        for (int d = LPK; d < 64; d <<= 1) {
+            sum += __shfl_xor(sum, d);
+#pragma unroll
+            for (int f = 0; f < NF; ++f)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[t][f][e] += __shfl_xor(o[t][f][e], d);
+        }
+        if (lane < LPK) {
+#pragma unroll
+            for (int f = 0; f < NF; ++f) *reinterpret_cast<floatx4*>(&join_o[wave][t][4 * (sub + LPK * f)]) = o[t][f];
+            if (lane == 0) {
+                join_ml[wave][t][0] = top;
+                join_ml[wave][t][1] = sum;
+            }
+        }
+    }
+    __syncthreads();
+    const Partials part = partials(ws, gridDim.y, kv, gridDim.x, w.item0 + w.range, RT, dim);
+    for (int e = threadIdx.x; e < RT * (W / 4); e += 256) {
+        const int t = e / (W / 4), d = 4 * (e % (W / 4)), rho = rho0 + t;
+        if (rho >= rows) continue;
+        float top = -INFINITY;
+        for (int i = 0; i < 4; ++i) top = fmaxf(top, join_ml[i][t][0]);
+        const float base = top == -INFINITY ? 0.f : top;
+        float sum = 0.f;
+        floatx4 x = {0.f, 0.f, 0.f, 0.f};
+        for (int i = 0; i < 4; ++i) {
+            const float corr = exp2f(join_ml[i][t][0] - base);
+            sum += join_ml[i][t][1] * corr;
+            x += *reinterpret_cast<const floatx4*>(&join_o[i][t][d]) * corr;
+        }
+        const size_t head = (size_t)kv * group + rho % group, row = sp.q0 + rho / group;
+        const size_t at = head * a.q_rows + row;
+        if (tl.ranges == 1) {
+            const float inv = rho / group + shift < 0 || sp.kl == 0 ? 0.f : 1.0f / sum;
+            store4(out + row * a.o_rs + head * dim, d, dim, a.vec, x * inv);
+            if (lse && d == 0) lse[at] = (top + log2f(sum)) * kLn2;
+        } else {
+            store4(part.o + t * dim, d, dim, false, x);
+            if (d == 0) {
+                part.ml[2 * t] = top;
+                part.ml[2 * t + 1] = sum;
+            }
+        }
+    }
+}
+
+// Joins the ranges of the rows whose keys were cut into more than one: a wave per row, four rows of a
+// tile per work-group; the ranges' outputs are added in range order.
+template <int TILE>
+__global__ __launch_bounds__(256) void attn_packed_join_kernel(PackedAttn a, float* __restrict__ out, float* __restrict__ lse,
+                                                               float* __restrict__ ws, uint32_t budget, uint32_t items) {
+    Work w;
+    if (!find_work<false, true>(a, TILE, budget, blockIdx.x, &w)) return;
+    const RowTile tl = row_tile(a, w, TILE);
+    const int lane = threadIdx.x & 63, t = blockIdx.z * 4 + (threadIdx.x >> 6), rho = tl.rho0 + t;
+    if (tl.ranges == 1 || rho > tl.last) return;
+    const int dim = a.head_dim, group = a.group, kv = blockIdx.y;
+    const size_t head = (size_t)kv * group + rho % group, row = w.sp.q0 + rho / group;
+    const Partials part = partials(ws, gridDim.y, kv, items, w.item0, TILE, dim);
+    float top = -INFINITY;
+    for (int z = lane; z < tl.ranges; z += 64) top = fmaxf(top, part.ml[2 * (z * TILE + t)]);
+    top = wave_max(top);
+    const float base = top == -INFINITY ? 0.f : top;
+    float sum = 0.f, x[2] = {0.f, 0.f};
+    for (int z0 = 0; z0 < tl.ranges; z0 += 64) {
+        const int z = z0 + lane;
+        float corr = 0.f;
+        if (z < tl.ranges) {
+            corr = exp2f(part.ml[2 * (z * TILE + t)] - base);
+            sum += part.ml[2 * (z * TILE + t) + 1] * corr;
+        }
+        const int n = min(64, tl.ranges - z0);
+        for (int i0 = 0; i0 < n; i0 += 8) {
+            float y[8][2];
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                    y[i][e] = lane + 64 * e < dim ? part.o[((size_t)min(z0 + i0 + i, tl.ranges - 1) * TILE + t) * dim + lane + 64 * e] : 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float c = __shfl(corr, i0 + i);
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                    if (i0 + i < n) x[e] += y[i][e] * c;
+            }
+        }
+    }
+    sum = wave_sum(sum);
+    const float inv = rho / group + tl.shift < 0 ? 0.f : 1.0f / sum;
+    float* dst = out + row * a.o_rs + head * dim;
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+        if (lane + 64 * e < dim) dst[lane + 64 * e] = x[e] * inv;
+    if (lse && lane == 0) lse[head * a.q_rows + row] = (top + log2f(sum)) * kLn2;
 }
 
 // ---- forward ---------------------------------------------------------------------------------
@@ -191,26 +291,23 @@ __device__ __forceinline__ void add_seen(floatx16 (&acc)[DP / 32], const float* 
 template <int DP>
 __global__ __launch_bounds__(256) void attn_packed_kernel(PackedAttn a, float* __restrict__ out, float* __restrict__ lse,
                                                           const float* __restrict__ q, const float* __restrict__ k,
-                                                          const float* __restrict__ v) {
+                                                          const float* __restrict__ v, float* __restrict__ ws, uint32_t budget) {
     constexpr int KT = 32, KL = DP + 4, VL = DP + 8;
     __shared__ __attribute__((aligned(16))) float ks[KT * KL];
     __shared__ __attribute__((aligned(16))) float vs[KT * VL];
     __shared__ int bad_tile;  // the last tile whose values are not all finite, + 1
-    Span sp;
-    uint32_t tile, tiles;
-    if (!find_tile<false>(a, kRowsPerWG, blockIdx.x, &sp, &tile, &tiles)) return;
-    tile = tiles - 1 - tile;  // longest first
+    const int kv = blockIdx.x % a.n_kv;
+    Work w;
+    if (!find_work<false, false>(a, kRowsPerWG, budget, blockIdx.x / a.n_kv, &w)) return;
+    const RowTile tl = row_tile(a, w, kRowsPerWG);
+    if (w.range >= tl.ranges) return;
+    const Span sp = w.sp;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, c = lane & 31;
-    const int dim = a.head_dim, group = a.group, kv = blockIdx.y;
-    const uint32_t rows = sp.ql * group;
-    const uint32_t rho0 = tile * kRowsPerWG, rho = rho0 + wave * kRowsPerWave + c;
+    const int dim = a.head_dim, group = a.group, rows = tl.rows, shift = tl.shift, k_begin = tl.k_begin, k_end = tl.k_end;
+    const int rho = tl.rho0 + wave * kRowsPerWave + c;
     const bool live = rho < rows;
-    const uint32_t qi = (live ? rho : rows - 1) / group;
-    const int head = kv * group + (live ? rho : rows - 1) % group;
-    const int shift = (int)sp.kl - (int)sp.ql;
-    const int limit = (int)qi + shift;  // last key this row sees
-    const uint32_t last_qi = min(rho0 + kRowsPerWG - 1, rows - 1) / group;
-    const int nkeys = min((int)last_qi + shift + 1, (int)sp.kl);  // keys the work-group needs
+    const int qi = (live ? rho : rows - 1) / group, head = kv * group + (live ? rho : rows - 1) % group;
+    const int limit = qi + shift;  // last key this row sees
     const float* kb = k + (size_t)sp.k0 * a.k_rs + (size_t)kv * a.k_hs;
     const float* vb = v + (size_t)sp.k0 * a.v_rs + (size_t)kv * a.v_hs;
 
@@ -230,18 +327,18 @@ __global__ __launch_bounds__(256) void attn_packed_kernel(PackedAttn a, float* _
     float m = -INFINITY, l = 0.f;
     const float factor = a.scale * kLog2e;
     if (threadIdx.x == 0) bad_tile = 0;
-    for (int t0 = 0; t0 < nkeys; t0 += KT) {
+    for (int t0 = k_begin; t0 < k_end; t0 += KT) {
         __syncthreads();
-        stage_rows<KT, DP, KL>(ks, kb, a.k_rs, t0, nkeys, dim, a.vec);
-        if (stage_rows<KT, DP, VL>(vs, vb, a.v_rs, t0, nkeys, dim, a.vec) != 0.f) bad_tile = t0 + 1;
+        stage_rows<KT, DP, KL>(ks, kb, a.k_rs, t0, k_end, dim, a.vec);
+        if (stage_rows<KT, DP, VL>(vs, vb, a.v_rs, t0, k_end, dim, a.vec) != 0.f) bad_tile = t0 + 1;
         __syncthreads();
-        floatx16 s = rows_product<DP, KL>(ks, qr, h, c);
+        floatx16 s = lds_rows_product<DP, KL>(ks, qr, h, c);
         uint32_t seen = 0;
         float top = m;
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
             s[r] *= factor;
-            if (t0 + acc_row(r, h) <= limit) {
+            if (t0 + acc_row(r, h) <= min(limit, k_end - 1)) {
                 seen |= 1u << r;
                 top = fmaxf(top, s[r]);
             } else {
@@ -263,13 +360,28 @@ __global__ __launch_bounds__(256) void attn_packed_kernel(PackedAttn a, float* _
         for (int i = 0; i < DP / 32; ++i)
 #pragma unroll
             for (int r = 0; r < 16; ++r) o[i][r] *= corr;
-        if (bad_tile == t0 + 1 && __ballot(seen != 0xffffu)) add_seen<DP, VL>(o, vs, s, seen, h, c);
+        if (bad_tile == t0 + 1 && __ballot(seen != 0xffffu)) add_seen<DP>(o, s, seen, h, c, DP, true, [&](int n) { return vs + n * VL; });
         else add_product<DP, VL>(o, vs, s, h, c);
     }
     l += __shfl_xor(l, 32);
     if (!live) return;
-    const float inv = limit < 0 || sp.kl == 0 ? 0.f : 1.0f / l;
+    const size_t at = (size_t)head * a.q_rows + sp.q0 + qi;
+    float inv = limit < 0 || sp.kl == 0 ? 0.f : 1.0f / l;
     float* dst = out + (size_t)(sp.q0 + qi) * a.o_rs + (size_t)head * dim;
+    int vec = a.vec;
+    if (tl.ranges > 1) {
+        const int t = rho - tl.rho0;
+        const Partials part = partials(ws, a.n_kv, kv, gridDim.x / a.n_kv, w.item0 + w.range, kRowsPerWG, dim);
+        inv = 1.0f;
+        dst = part.o + t * dim;
+        vec = 0;
+        if (h == 0) {
+            part.ml[2 * t] = m;
+            part.ml[2 * t + 1] = l;
+        }
+    } else if (lse && h == 0) {
+        lse[at] = (m + log2f(l)) * kLn2;
+    }
 #pragma unroll
     for (int i = 0; i < DP / 32; ++i)
 #pragma unroll
@@ -277,9 +389,8 @@ __global__ __launch_bounds__(256) void attn_packed_kernel(PackedAttn a, float* _
             floatx4 x;
 #pragma unroll
             for (int e = 0; e < 4; ++e) x[e] = o[i][4 * u + e] * inv;
-            store4(dst, 32 * i + 8 * u + 4 * h, dim, a.vec, x);
+            store4(dst, 32 * i + 8 * u + 4 * h, dim, vec, x);
         }
-    if (lse && h == 0) lse[(size_t)head * a.q_rows + sp.q0 + qi] = (m + log2f(l)) * kLn2;
 }
 
 // ---- backward --------------------------------------------------------------------------------
@@ -295,21 +406,17 @@ __global__ __launch_bounds__(256) void attn_packed_dq_kernel(PackedAttn a, float
     __shared__ __attribute__((aligned(16))) float ks[KT * LD];
     __shared__ __attribute__((aligned(16))) float vs[KT * LD];
     __shared__ int bad_tile;
-    Span sp;
-    uint32_t tile, tiles;
-    if (!find_tile<false>(a, kRowsPerWG, blockIdx.x, &sp, &tile, &tiles)) return;
-    tile = tiles - 1 - tile;
+    const int kv = blockIdx.x % a.n_kv;
+    Work w;
+    if (!find_work<false, true>(a, kRowsPerWG, 0, blockIdx.x / a.n_kv, &w)) return;
+    const RowTile tl = row_tile(a, w, kRowsPerWG);
+    const Span sp = w.sp;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, c = lane & 31;
-    const int dim = a.head_dim, group = a.group, kv = blockIdx.y;
-    const uint32_t rows = sp.ql * group;
-    const uint32_t rho0 = tile * kRowsPerWG, rho = rho0 + wave * kRowsPerWave + c;
+    const int dim = a.head_dim, group = a.group, rows = tl.rows, shift = tl.shift, nkeys = tl.nkeys;
+    const int rho = tl.rho0 + wave * kRowsPerWave + c;
     const bool live = rho < rows;
-    const uint32_t qi = (live ? rho : rows - 1) / group;
-    const int head = kv * group + (live ? rho : rows - 1) % group;
-    const int shift = (int)sp.kl - (int)sp.ql;
-    const int limit = (int)qi + shift;
-    const uint32_t last_qi = min(rho0 + kRowsPerWG - 1, rows - 1) / group;
-    const int nkeys = min((int)last_qi + shift + 1, (int)sp.kl);
+    const int qi = (live ? rho : rows - 1) / group, head = kv * group + (live ? rho : rows - 1) % group;
+    const int limit = qi + shift;  // last key this row sees
     const float* kb = k + (size_t)sp.k0 * a.k_rs + (size_t)kv * a.k_hs;
     const float* vb = v + (size_t)sp.k0 * a.v_rs + (size_t)kv * a.v_hs;
 
@@ -345,8 +452,8 @@ __global__ __launch_bounds__(256) void attn_packed_dq_kernel(PackedAttn a, float
         if (stage_rows<KT, DP, LD>(ks, kb, a.k_rs, t0, nkeys, dim, a.vec) != 0.f) bad_tile = t0 + 1;
         stage_rows<KT, DP, LD>(vs, vb, a.v_rs, t0, nkeys, dim, a.vec);
         __syncthreads();
-        const floatx16 s = rows_product<DP, LD>(ks, qr, h, c);
-        floatx16 ds = rows_product<DP, LD>(vs, gr, h, c);
+        const floatx16 s = lds_rows_product<DP, LD>(ks, qr, h, c);
+        floatx16 ds = lds_rows_product<DP, LD>(vs, gr, h, c);
         uint32_t seen = 0;
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
@@ -354,7 +461,7 @@ __global__ __launch_bounds__(256) void attn_packed_dq_kernel(PackedAttn a, float
             ds[r] = on ? exp2f(s[r] * factor - lse2) * (ds[r] - d) * a.scale : 0.f;
             seen |= (on ? 1u : 0u) << r;
         }
-        if (bad_tile == t0 + 1 && __ballot(seen != 0xffffu)) add_seen<DP, LD>(acc, ks, ds, seen, h, c);
+        if (bad_tile == t0 + 1 && __ballot(seen != 0xffffu)) add_seen<DP>(acc, ds, seen, h, c, DP, true, [&](int n) { return ks + n * LD; });
         else add_product<DP, LD>(acc, ks, ds, h, c);
     }
     if (!live) return;
@@ -380,11 +487,13 @@ __global__ __launch_bounds__(256) void attn_packed_dkv_kernel(PackedAttn a, floa
     __shared__ __attribute__((aligned(16))) float gs[RT * LD];
     __shared__ __attribute__((aligned(16))) float stats[2][RT];
     __shared__ int bad_tile;
-    Span sp;
-    uint32_t tile, tiles;
-    if (!find_tile<true>(a, kRowsPerWG, blockIdx.x, &sp, &tile, &tiles)) return;
+    const int kv = blockIdx.x % a.n_kv;
+    Work w;
+    if (!find_work<true, true>(a, kRowsPerWG, 0, blockIdx.x / a.n_kv, &w)) return;
+    const Span sp = w.sp;
+    const int tile = w.tile;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, c = lane & 31;
-    const int dim = a.head_dim, group = a.group, kv = blockIdx.y;
+    const int dim = a.head_dim, group = a.group;
     const int key = tile * kRowsPerWG + wave * kRowsPerWave + c;
     const bool live = key < (int)sp.kl;
     const int shift = (int)sp.kl - (int)sp.ql;
@@ -408,7 +517,7 @@ __global__ __launch_bounds__(256) void attn_packed_dkv_kernel(PackedAttn a, floa
         for (int r = 0; r < 16; ++r) ak[i][r] = av[i][r] = 0.f;
     const float factor = a.scale * kLog2e;
     if (threadIdx.x == 0) bad_tile = 0;
-    const int first = max(0, (int)tile * kRowsPerWG - shift) / RT * RT;  // the first row that sees a key of the tile
+    const int first = max(0, tile * kRowsPerWG - shift) / RT * RT;  // the first row that sees a key of the tile
     int pass = 0;
     for (int g = 0; g < group; ++g) {
         const int head = kv * group + g;
@@ -427,8 +536,8 @@ __global__ __launch_bounds__(256) void attn_packed_dkv_kernel(PackedAttn a, floa
             }
             if (bad != 0.f) bad_tile = pass;
             __syncthreads();
-            floatx16 p = rows_product<DP, LD>(qs, kr, h, c);
-            floatx16 ds = rows_product<DP, LD>(gs, vr, h, c);
+            floatx16 p = lds_rows_product<DP, LD>(qs, kr, h, c);
+            floatx16 ds = lds_rows_product<DP, LD>(gs, vr, h, c);
             uint32_t seen = 0;
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
@@ -439,8 +548,8 @@ __global__ __launch_bounds__(256) void attn_packed_dkv_kernel(PackedAttn a, floa
                 seen |= (on ? 1u : 0u) << r;
             }
             if (bad_tile == pass && __ballot(seen != 0xffffu)) {
-                add_seen<DP, LD>(av, gs, p, seen, h, c);
-                add_seen<DP, LD>(ak, qs, ds, seen, h, c);
+                add_seen<DP>(av, p, seen, h, c, DP, true, [&](int n) { return gs + n * LD; });
+                add_seen<DP>(ak, ds, seen, h, c, DP, true, [&](int n) { return qs + n * LD; });
             } else {
                 add_product<DP, LD>(av, gs, p, h, c);
                 add_product<DP, LD>(ak, qs, ds, h, c);
@@ -495,6 +604,7 @@ PackedAttn make_args(const fmlh_packed_attention* s) {
     a.q_rows = s->q_rows;
     a.k_rows = s->k_rows;
     a.group = s->n_head / s->n_kv_head;
+    a.n_kv = s->n_kv_head;
     a.head_dim = s->head_dim;
     a.scale = s->scale;
     a.q_off = s->q_off;
@@ -511,11 +621,36 @@ PackedAttn make_args(const fmlh_packed_attention* s) {
     return a;
 }
 
-uint32_t row_tiles(const PackedAttn& a) { return (uint32_t)(((uint64_t)a.q_rows * a.group) / kRowsPerWG) + a.n_seq; }
+uint32_t row_tiles(const PackedAttn& a, uint32_t per) { return (uint32_t)(((uint64_t)a.q_rows * a.group) / per) + a.n_seq; }
 uint32_t key_tiles(const PackedAttn& a) { return a.k_rows / kRowsPerWG + a.n_seq; }
 
-size_t workspace(const PackedAttn& a, uint32_t n_head, bool backward) {
-    return backward ? (size_t)n_head * a.q_rows : 0;  // d_i
+// How the forward pass cuts its work, by the sizes alone (lengths are the device's to know).
+struct ForwardPlan {
+    int per;          // rows per tile: kRowsPerWG, or at most 8 for attn_packed_few_kernel
+    uint32_t tiles;   // at most, for a key head
+    uint32_t budget;  // ranges to cut the tiles' keys into, for a key head; 0: none
+};
+
+ForwardPlan plan_forward(const PackedAttn& a) {
+    ForwardPlan p;
+    const uint64_t rows = (uint64_t)a.q_rows * a.group;  // of a key head
+    const uint64_t per_seq = rows / a.n_seq;
+    p.per = per_seq > 8 ? kRowsPerWG : per_seq > 4 ? 8 : per_seq > 2 ? 4 : per_seq > 1 ? 2 : 1;
+    p.tiles = row_tiles(a, p.per);
+    const uint64_t about = std::max<uint64_t>(a.n_seq, (rows + p.per - 1) / p.per) * a.n_kv;
+    const uint64_t want = p.per <= 8 ? 1024 : 512;  // work-groups that keep the device busy
+    p.budget = 2 * about <= want && a.k_rows > kRangeKeys ? (uint32_t)(want / a.n_kv) : 0;
+    return p;
+}
+
+// Work-groups of a launch, all key heads': its threads stay inside 32 bits.
+constexpr uint64_t kMaxGroups = 1u << 23;
+
+size_t workspace(const PackedAttn& a, bool backward) {
+    if (a.n_seq == 0) return 0;
+    const ForwardPlan p = plan_forward(a);
+    const size_t forward = p.budget ? (size_t)a.n_kv * (p.tiles + p.budget) * p.per * (a.head_dim + 2) : 0;
+    return backward ? std::max(forward, (size_t)a.n_kv * a.group * a.q_rows) : forward;  // backward: d_i
 }
 
 }  // namespace
@@ -537,7 +672,7 @@ extern "C" {
 int fmlh_attention_packed_workspace(const fmlh_packed_attention* shape, int backward, size_t* floats) {
     FMLH_REQUIRE(floats != nullptr, "fmlh_attention_packed_workspace: null output pointer");
     FMLH_TRY(check_shape("fmlh_attention_packed_workspace", shape));
-    *floats = workspace(make_args(shape), shape->n_head, backward != 0);
+    *floats = workspace(make_args(shape), backward != 0);
     return FMLH_OK;
 }
 
@@ -550,14 +685,52 @@ int fmlh_attention_packed(const fmlh_packed_attention* shape, float* out, float*
     FMLH_REQUIRE(shape->k_rows == 0 || (k && v), "%s: null keys or values", fn);
     FMLH_TRY(ensure_init());
     PackedAttn a = make_args(shape);
-    const size_t need = workspace(a, shape->n_head, false);
+    const size_t need = workspace(a, false);
     FMLH_REQUIRE(need == 0 || (ws && ws_floats >= need), "%s: a workspace of %zu floats is needed", fn, need);
     a.vec = a.vec && aligned16(q) && aligned16(k) && aligned16(v) && aligned16(out);
-    const dim3 grid(row_tiles(a), shape->n_kv_head);
-#define FMLH_LAUNCH(DP) hipLaunchKernelGGL(attn_packed_kernel<DP>, grid, dim3(256), 0, stream(), a, out, lse, q, k, v)
-    FMLH_BY_DIM(FMLH_LAUNCH);
+    const ForwardPlan plan = plan_forward(a);
+    const uint32_t items = plan.tiles + plan.budget;
+    FMLH_REQUIRE((uint64_t)items * a.n_kv <= kMaxGroups, "%s: more than 2^23 tiles of rows", fn);
+    if (plan.per <= 8) {
+        const dim3 grid(items, a.n_kv);
+#define FMLH_FEW(LPK, NF, RT) \
+    hipLaunchKernelGGL((attn_packed_few_kernel<LPK, NF, RT>), grid, dim3(256), 0, stream(), a, out, lse, q, k, v, ws, plan.budget)
+#define FMLH_FEW_ROWS(LPK, NF)                       \
+    do {                                             \
+        if (plan.per == 1) FMLH_FEW(LPK, NF, 1);      \
+        else if (plan.per == 2) FMLH_FEW(LPK, NF, 2); \
+        else if (plan.per == 4) FMLH_FEW(LPK, NF, 4); \
+        else FMLH_FEW(LPK, NF, 8);                    \
+    } while (0)
+        if (a.head_dim <= 16) FMLH_FEW_ROWS(4, 1);
+        else if (a.head_dim <= 32) FMLH_FEW_ROWS(8, 1);
+        else if (a.head_dim <= 64) FMLH_FEW_ROWS(16, 1);
+        else FMLH_FEW_ROWS(16, 2);
+#undef FMLH_FEW_ROWS
+#undef FMLH_FEW
+        FMLH_LAUNCHED("attn_packed_few_kernel");
+    } else {
+#define FMLH_LAUNCH(DP)                                                                                                \
+    hipLaunchKernelGGL(attn_packed_kernel<DP>, dim3(items * a.n_kv), dim3(256), 0, stream(), a, out, lse, q, k, v, ws, \
+                       plan.budget)
+        FMLH_BY_DIM(FMLH_LAUNCH);
 #undef FMLH_LAUNCH
-    FMLH_LAUNCHED("attn_packed_kernel");
+        FMLH_LAUNCHED("attn_packed_kernel");
+    }
+    if (plan.budget) {
+#define FMLH_JOIN(TILE)                                                                                                      \
+    hipLaunchKernelGGL(attn_packed_join_kernel<TILE>, dim3(plan.tiles, a.n_kv, (TILE + 3) / 4), dim3(256), 0, stream(), a, out, \
+                       lse, ws, plan.budget, items)
+        switch (plan.per) {
+            case 1: FMLH_JOIN(1); break;
+            case 2: FMLH_JOIN(2); break;
+            case 4: FMLH_JOIN(4); break;
+            case 8: FMLH_JOIN(8); break;
+            default: FMLH_JOIN(kRowsPerWG); break;
+        }
+#undef FMLH_JOIN
+        FMLH_LAUNCHED("attn_packed_join_kernel");
+    }
     return FMLH_OK;
 }
 
@@ -571,12 +744,13 @@ int fmlh_attention_packed_backward(const fmlh_packed_attention* shape, float* dq
     FMLH_REQUIRE(shape->k_rows == 0 || (dk && dv && k && v), "%s: null pointer", fn);
     FMLH_TRY(ensure_init());
     PackedAttn a = make_args(shape);
-    const size_t need = workspace(a, shape->n_head, true);
+    const size_t need = (size_t)shape->n_head * shape->q_rows;
     FMLH_REQUIRE(need == 0 || (ws && ws_floats >= need), "%s: a workspace of %zu floats is needed", fn, need);
+    FMLH_REQUIRE((uint64_t)std::max(row_tiles(a, kRowsPerWG), key_tiles(a)) * a.n_kv <= kMaxGroups, "%s: more than 2^23 tiles of rows or keys", fn);
     a.vec = a.vec && aligned16(q) && aligned16(k) && aligned16(v) && aligned16(out) && aligned16(dout) && aligned16(dq) &&
             aligned16(dk) && aligned16(dv);
     if (shape->q_rows) {
-        const dim3 grid(row_tiles(a), shape->n_kv_head);
+        const dim3 grid(row_tiles(a, kRowsPerWG) * a.n_kv);
 #define FMLH_LAUNCH(DP) \
     hipLaunchKernelGGL(attn_packed_dq_kernel<DP>, grid, dim3(256), 0, stream(), a, dq, ws, dout, out, lse, q, k, v)
         FMLH_BY_DIM(FMLH_LAUNCH);
@@ -584,7 +758,7 @@ int fmlh_attention_packed_backward(const fmlh_packed_attention* shape, float* dq
         FMLH_LAUNCHED("attn_packed_dq_kernel");
     }
     if (shape->k_rows) {
-        const dim3 grid(key_tiles(a), shape->n_kv_head);
+        const dim3 grid(key_tiles(a) * a.n_kv);
 #define FMLH_LAUNCH(DP) \
     hipLaunchKernelGGL(attn_packed_dkv_kernel<DP>, grid, dim3(256), 0, stream(), a, dk, dv, ws, dout, lse, q, k, v)
         FMLH_BY_DIM(FMLH_LAUNCH);

@@ -287,8 +287,8 @@ typedef struct fmlh_packed_attention {
     size_t k_hs, v_hs;             /* head strides of k and v, in floats */
 } fmlh_packed_attention;
 
-/* Floats of device workspace that a forward (backward = 0) or backward call of this shape needs; 0:
- * none.  It depends on the sizes alone, not on the offsets' contents.  A workspace serves one call
+/* Floats of device workspace that a forward call of this shape needs (backward = 0; 0 floats: none),
+ * or enough for the forward and the backward call (backward = 1).  It depends on the sizes alone, not on the offsets' contents.  A workspace serves one call
  * at a time: calls and captured graphs that may run at once need one each. */
 int fmlh_attention_packed_workspace(const fmlh_packed_attention* shape, int backward, size_t* floats);
 
