@@ -16,4 +16,15 @@ struct PackedAttn {
     size_t q_rs, k_rs, v_rs, o_rs, k_hs, v_hs;
 };
 
+// The kernels on the bf16 matrix cores (attention_packed_split.hip).  Grids hold `items` / `tiles` per
+// key head; ws and part are workspace.
+int attn_split_forward(const PackedAttn& a, uint32_t items, uint32_t budget, float* out, float* lse, const float* q, const float* k,
+                       const float* v, float* ws, hipStream_t s);
+int attn_split_dq(const PackedAttn& a, uint32_t tiles, float* dq, float* delta, const float* dout, const float* out, const float* lse,
+                  const float* q, const float* k, const float* v, hipStream_t s);
+// Floats that one of the parts of attn_split_dkv leaves (parts > 1).
+size_t attn_split_part_floats(const PackedAttn& a, uint32_t tiles);
+int attn_split_dkv(const PackedAttn& a, uint32_t tiles, int parts, float* dk, float* dv, const float* delta, const float* dout,
+                   const float* lse, const float* q, const float* k, const float* v, float* part, hipStream_t s);
+
 }  // namespace fmlh

@@ -646,11 +646,24 @@ ForwardPlan plan_forward(const PackedAttn& a) {
 // Work-groups of a launch, all key heads': its threads stay inside 32 bits.
 constexpr uint64_t kMaxGroups = 1u << 23;
 
+// How the backward pass cuts the rows that a tile of keys sees.
+int plan_parts(const PackedAttn& a) {
+    const uint64_t tiles = std::max<uint64_t>(std::min(a.n_seq, key_tiles(a)), a.k_rows / kRowsPerWG) * a.n_kv;
+    const uint64_t want = 1024;          // work-groups that keep the device busy although early keys see more rows than late ones
+    const size_t most = size_t(1) << 26;  // floats of partial sums
+    const uint64_t fit = std::max<uint64_t>(1, most / std::max<size_t>(1, attn_split_part_floats(a, key_tiles(a))));
+    return (int)std::min<uint64_t>({16, fit, std::max<uint64_t>(1, want / std::max<uint64_t>(1, tiles))});
+}
+
+size_t deltas(const PackedAttn& a) { return ((size_t)a.n_kv * a.group * a.q_rows + 3) / 4 * 4; }  // d_i, in whole 16 bytes
+
 size_t workspace(const PackedAttn& a, bool backward) {
     if (a.n_seq == 0) return 0;
     const ForwardPlan p = plan_forward(a);
     const size_t forward = p.budget ? (size_t)a.n_kv * (p.tiles + p.budget) * p.per * (a.head_dim + 2) : 0;
-    return backward ? std::max(forward, (size_t)a.n_kv * a.group * a.q_rows) : forward;  // backward: d_i
+    if (!backward) return forward;
+    const int parts = plan_parts(a);
+    return std::max(forward, deltas(a) + (parts > 1 ? parts * attn_split_part_floats(a, key_tiles(a)) : 0));
 }
 
 }  // namespace
@@ -709,6 +722,8 @@ int fmlh_attention_packed(const fmlh_packed_attention* shape, float* out, float*
 #undef FMLH_FEW_ROWS
 #undef FMLH_FEW
         FMLH_LAUNCHED("attn_packed_few_kernel");
+    } else if (!getenv("FMLH_PLAIN")) {
+        FMLH_TRY(attn_split_forward(a, items, plan.budget, out, lse, q, k, v, ws, stream()));
     } else {
 #define FMLH_LAUNCH(DP)                                                                                                \
     hipLaunchKernelGGL(attn_packed_kernel<DP>, dim3(items * a.n_kv), dim3(256), 0, stream(), a, out, lse, q, k, v, ws, \
@@ -744,11 +759,18 @@ int fmlh_attention_packed_backward(const fmlh_packed_attention* shape, float* dq
     FMLH_REQUIRE(shape->k_rows == 0 || (dk && dv && k && v), "%s: null pointer", fn);
     FMLH_TRY(ensure_init());
     PackedAttn a = make_args(shape);
-    const size_t need = (size_t)shape->n_head * shape->q_rows;
+    const int parts = plan_parts(a);
+    const size_t need = deltas(a) + (parts > 1 ? parts * attn_split_part_floats(a, key_tiles(a)) : 0);
     FMLH_REQUIRE(need == 0 || (ws && ws_floats >= need), "%s: a workspace of %zu floats is needed", fn, need);
     FMLH_REQUIRE((uint64_t)std::max(row_tiles(a, kRowsPerWG), key_tiles(a)) * a.n_kv <= kMaxGroups, "%s: more than 2^23 tiles of rows or keys", fn);
     a.vec = a.vec && aligned16(q) && aligned16(k) && aligned16(v) && aligned16(out) && aligned16(dout) && aligned16(dq) &&
             aligned16(dk) && aligned16(dv);
+    FMLH_REQUIRE((uintptr_t)ws % 16 == 0, "%s: the workspace is not 16-byte aligned", fn);
+    if (!getenv("FMLH_PLAIN")) {
+        if (shape->q_rows) FMLH_TRY(attn_split_dq(a, row_tiles(a, kRowsPerWG), dq, ws, dout, out, lse, q, k, v, stream()));
+        if (shape->k_rows) FMLH_TRY(attn_split_dkv(a, key_tiles(a), parts, dk, dv, ws, dout, lse, q, k, v, ws + deltas(a), stream()));
+        return FMLH_OK;
+    }
     if (shape->q_rows) {
         const dim3 grid(row_tiles(a, kRowsPerWG) * a.n_kv);
 #define FMLH_LAUNCH(DP) \

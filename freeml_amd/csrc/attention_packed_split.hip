@@ -1,0 +1,615 @@
+// The packed attention kernels on the bf16 matrix cores: forward, dq, and dk / dv (attention_packed.hip
+// has the formulas and the layout of tiles and lanes).
+//
+// Every operand is written exactly as three bf16 parts (bf16_split.h) and the six part products of
+// weight 2^-16 and more are summed in fp32 by v_mfma_f32_32x32x16_bf16: 6 x 32 clocks per 32 x 32 x 16
+// block where the fp32 matrix cores need 512.
+//   * Operands are staged times 2^24, so that every part of every fp32 number is zero or normal; sums
+//     carry 2^48 and are taken back.  What leaves the range at the upper end (elements from 2^104, sums
+//     from 2^80), and infinities and NaN, masked ones included, show as a result that is not finite:
+//     that wave does its rows or keys again, on the fp32 matrix cores and element by element, from memory.
+//   * A tile's rows lie in LDS as bf16 planes, 16-byte units of 8 dims: unit o of row r at o ^ swz(r), so
+//     that 8 lanes on one unit of 8 rows touch distinct banks.  Products over the dims read them by
+//     row; products over the rows read them transposed (ds_read_b64_tr_b16: lanes 4 r .. 4 r + 3 of 16
+//     name 16 dims of row r, lane i gets dim i of 4 rows), so one copy serves both.
+//   * A lane's accumulator registers 8 t .. 8 t + 7 are rows 16 t + 4 h + {0..3, 8..11} of its column:
+//     taking the rows in this order as the 8 k of a half makes probabilities and their gradients
+//     the next product's operand without leaving the registers.
+//   * A tile's rows are requested into registers while the tile before them is multiplied.
+#include "attention_packed_device.h"
+
+namespace fmlh {
+
+namespace {
+
+constexpr float kUp = 0x1p24f, kDown2 = 0x1p-48f;
+
+template <int DP>
+struct Shape {
+    static constexpr int U = DP / 8;      // 16-byte units per row and plane
+    static constexpr int KS = DP / 16;    // steps of a product over the dims
+    static constexpr int NB = DP / 32;    // blocks of 32 dims
+    __device__ static __forceinline__ int swz(int r) { return U % 8 == 0 ? (r & 7) : ((r >> 2) & 3); }
+};
+
+// R rows of a matrix in registers (a thread's share) and from there as planes in LDS.
+template <int R, int DP>
+struct Stage {
+    static constexpr int U = DP / 8, N = (R * U + 255) / 256;
+    floatx4 x[N][2];
+    // Rows first .. of a matrix at base, row stride rs; rows from `rows` on are zeros.
+    __device__ __forceinline__ void load(const float* base, size_t rs, int first, int rows, int dim, bool vec) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int u = threadIdx.x + 256 * i, r = first + u / U, d = 8 * (u % U);
+            x[i][0] = x[i][1] = floatx4{0.f, 0.f, 0.f, 0.f};
+            if (r < rows && (R * U % 256 == 0 || u < R * U)) {
+                const float* row = base + (size_t)r * rs;
+                x[i][0] = load4(row, d, dim, vec);
+                x[i][1] = load4(row, d + 4, dim, vec);
+            }
+        }
+    }
+    __device__ __forceinline__ void store(uintx4* planes) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int u = threadIdx.x + 256 * i, r = u / U;
+            if (R * U % 256 != 0 && u >= R * U) break;
+            const float v[8] = {x[i][0][0], x[i][0][1], x[i][0][2], x[i][0][3], x[i][1][0], x[i][1][1], x[i][1][2], x[i][1][3]};
+            uintx4 p[3];
+            split8(v, p, kUp);
+#pragma unroll
+            for (int q = 0; q < 3; ++q) planes[(q * R + r) * U + ((u % U) ^ Shape<DP>::swz(r))] = p[q];
+        }
+    }
+};
+
+// Row `row` of a tile as the matrix core's operand of dims 16 st + 8 h ..
+template <int R, int DP>
+__device__ __forceinline__ bf16x8 row_operand(const uintx4* planes, int q, int row, int st, int h) {
+    constexpr int U = DP / 8;
+    return __builtin_bit_cast(bf16x8, planes[(q * R + row) * U + ((2 * st + h) ^ Shape<DP>::swz(row))]);
+}
+
+// Dim 32 i + lane % 32 of rows row0 + 4 h + {0..3, 8..11} of a tile.
+typedef short shortx4 __attribute__((ext_vector_type(4)));
+typedef short shortx8 __attribute__((ext_vector_type(8)));
+template <int R, int DP>
+__device__ __forceinline__ bf16x8 column_operand(const uintx4* planes, int q, int row0, int i, int lane) {
+    constexpr int U = DP / 8;
+    const int row = row0 + 4 * (lane >> 5) + ((lane & 15) >> 2);
+    const int unit = 4 * i + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+    typedef __attribute__((address_space(3))) shortx4 lds_shortx4;
+    auto at = [&](int r) {
+        return __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (lds_shortx4*)(planes + (q * R + r) * U + (unit ^ Shape<DP>::swz(r))) + (lane & 1));
+    };
+    const shortx4 lo = at(row), hi = at(row + 8);
+    return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
+// A lane's row as operand of products over the dims: dims 16 st + 8 h .. of every step, three parts.
+template <int DP>
+__device__ __forceinline__ void load_operand(bf16x8 (&p)[3][DP / 16], const float* row, int h, int dim, bool vec) {
+#pragma unroll
+    for (int st = 0; st < DP / 16; ++st) {
+        const floatx4 a = load4(row, 16 * st + 8 * h, dim, vec), b = load4(row, 16 * st + 8 * h + 4, dim, vec);
+        const float v[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+        uintx4 u[3];
+        split8(v, u, kUp);
+#pragma unroll
+        for (int q = 0; q < 3; ++q) p[q][st] = __builtin_bit_cast(bf16x8, u[q]);
+    }
+}
+
+// s (32 rows x 32 columns) = tile rows row0 .. row0 + 31 times the lanes' columns, over the dims.
+template <int R, int DP>
+__device__ __forceinline__ floatx16 tile_product(const uintx4* planes, int row0, const bf16x8 (&b)[3][DP / 16], int h, int c) {
+    floatx16 s;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] = 0.f;
+#pragma unroll
+    for (int st = 0; st < DP / 16; ++st) {
+        bf16x8 a[3];
+#pragma unroll
+        for (int q = 0; q < 3; ++q) a[q] = row_operand<R, DP>(planes, q, row0 + c, st, h);
+#pragma unroll
+        for (int q = 0; q < 6; ++q) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[kSplitA[q]], b[kSplitB[q]][st], s, 0, 0, 0);
+    }
+    return s;
+}
+
+// acc (dims x 32 columns) += (tile rows row0 .. row0 + 31)^T times their weights w, w times 2^24.
+template <int R, int DP>
+__device__ __forceinline__ void tile_add(floatx16 (&acc)[DP / 32], const uintx4* planes, int row0, const floatx16& w, int lane) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = w[8 * t + e];
+        uintx4 u[3];
+        split8(x, u, kUp);
+#pragma unroll
+        for (int i = 0; i < DP / 32; ++i) {
+            bf16x8 a[3];
+#pragma unroll
+            for (int q = 0; q < 3; ++q) a[q] = column_operand<R, DP>(planes, q, row0 + 16 * t, i, lane);
+#pragma unroll
+            for (int q = 0; q < 6; ++q)
+                acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[kSplitA[q]], __builtin_bit_cast(bf16x8, u[kSplitB[q]]), acc[i], 0, 0, 0);
+        }
+    }
+}
+
+// Whether a value of the wave's accumulators is infinite or NaN.
+template <int N>
+__device__ __forceinline__ bool any_not_finite(const floatx16 (&acc)[N]) {
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) bad |= !(fabsf(acc[i][r]) < INFINITY);
+    return __ballot(bad) != 0;
+}
+
+// LDS accesses of the work-group's waves are done; requested loads stay in flight.
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+__device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }  // below 2^-126: zero
+
+// ---- forward ---------------------------------------------------------------------------------
+
+template <int DP>
+__global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attn_split_kernel(PackedAttn a, float* __restrict__ out, float* __restrict__ lse,
+                                                            const float* __restrict__ q, const float* __restrict__ k,
+                                                            const float* __restrict__ v, float* __restrict__ ws, uint32_t budget) {
+    constexpr int KT = DP <= 64 ? 64 : 32, U = DP / 8, NB = DP / 32;
+    __shared__ uintx4 kp[3 * KT * U];
+    __shared__ uintx4 vp[3 * KT * U];
+    const int kv = blockIdx.x % a.n_kv;
+    Work w;
+    if (!find_work<false, false>(a, kRowsPerWG, budget, blockIdx.x / a.n_kv, &w)) return;
+    const RowTile tl = row_tile(a, w, kRowsPerWG);
+    if (w.range >= tl.ranges) return;
+    const Span sp = w.sp;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, c = lane & 31;
+    const int dim = a.head_dim, group = a.group, rows = tl.rows, shift = tl.shift, k_begin = tl.k_begin, k_end = tl.k_end;
+    const bool vec = a.vec;
+    const int rho0 = tl.rho0 + wave * kRowsPerWave, rho = rho0 + c;
+    const bool live = rho < rows;
+    const int qi = (live ? rho : rows - 1) / group, head = kv * group + (live ? rho : rows - 1) % group;
+    const int limit = min(qi + shift, k_end - 1);  // last key of the range that this row sees
+    // Over the wave's rows (uniform): the first row's limit, and the last one's.
+    const int first_limit = min(rho0, rows - 1) / group + shift, last_limit = min(rho0 + kRowsPerWave, rows) - 1 < rho0
+                                                                                  ? -1
+                                                                                  : (min(rho0 + kRowsPerWave, rows) - 1) / group + shift;
+    const float* kb = k + (size_t)sp.k0 * a.k_rs + (size_t)kv * a.k_hs;
+    const float* vb = v + (size_t)sp.k0 * a.v_rs + (size_t)kv * a.v_hs;
+    const float* q_row = q + (size_t)(sp.q0 + qi) * a.q_rs + (size_t)head * dim;
+
+    Stage<KT, DP> ks, vs;
+    ks.load(kb, a.k_rs, k_begin, k_end, dim, vec);
+    vs.load(vb, a.v_rs, k_begin, k_end, dim, vec);
+    bf16x8 qp[3][DP / 16];
+    load_operand<DP>(qp, q_row, h, dim, vec);
+    floatx16 o[NB];
+    clear(o);
+    float top = -INFINITY, l = 0.f;  // the running maximum of the raw products, the sum of exponentials
+    // A softmax step over 32 keys at t0 of products s, exponent factor f (its sign decides which product is largest).
+    auto softmax = [&](floatx16* s, int blocks, int t0, float f) {
+        const bool edge = t0 + 32 * blocks - 1 > min(first_limit, k_end - 1);
+        float mt = top;
+        for (int j = 0; j < blocks; ++j) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                s[j][r] *= f;
+                if (edge && t0 + 32 * j + acc_row(r, h) > limit) s[j][r] = -INFINITY;
+                mt = fmaxf(mt, s[j][r]);
+            }
+        }
+        mt = fmaxf(mt, __shfl_xor(mt, 32));
+        const float base = mt == -INFINITY ? 0.f : mt;
+        const float corr = fast_exp2(top - base);
+        top = mt;
+        float sum = 0.f;
+        for (int j = 0; j < blocks; ++j)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                s[j][r] = fast_exp2(s[j][r] - base);
+                sum += s[j][r];
+            }
+        l = l * corr + sum;
+        if (__ballot(corr != 1.0f)) {
+#pragma unroll
+            for (int i = 0; i < NB; ++i)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[i][r] *= corr;
+        }
+    };
+    const float factor = a.scale * kLog2e;
+    for (int t0 = k_begin; t0 < k_end; t0 += KT) {
+        lds_barrier();
+        ks.store(kp);
+        vs.store(vp);
+        if (t0 + KT < k_end) {
+            ks.load(kb, a.k_rs, t0 + KT, k_end, dim, vec);
+            vs.load(vb, a.v_rs, t0 + KT, k_end, dim, vec);
+        }
+        lds_barrier();
+        if (t0 > last_limit) continue;  // no row of the wave sees the tile
+        floatx16 s[KT / 32];
+#pragma unroll
+        for (int j = 0; j < KT / 32; ++j) s[j] = tile_product<KT, DP>(kp, 32 * j, qp, h, c);
+        softmax(s, KT / 32, t0, factor * kDown2);
+#pragma unroll
+        for (int j = 0; j < KT / 32; ++j) tile_add<KT, DP>(o, vp, 32 * j, s[j], lane);
+    }
+    float unit = kDown2;
+    if (any_not_finite(o)) {
+        clear(o);
+        top = -INFINITY;
+        l = 0.f;
+        unit = 1.0f;
+#pragma unroll 1
+        for (int t0 = k_begin; t0 < k_end && t0 <= last_limit; t0 += 32) {
+            const int lk = k_end - 1;
+            floatx16 s[1];
+            s[0] = rows_product<DP>(kb + (size_t)min(t0 + c, lk) * a.k_rs, q_row, dim, vec, h);
+            softmax(s, 1, t0, factor);
+            uint32_t seen = 0;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) seen |= (t0 + acc_row(r, h) <= limit ? 1u : 0u) << r;
+            add_seen<DP>(o, s[0], seen, h, c, dim, vec, [&](int n) { return vb + (size_t)min(t0 + n, lk) * a.v_rs; });
+        }
+    }
+    l += __shfl_xor(l, 32);
+    if (!live) return;
+    float inv = qi + shift < 0 || sp.kl == 0 ? 0.f : 1.0f / l;
+    float* dst = out + (size_t)(sp.q0 + qi) * a.o_rs + (size_t)head * dim;
+    bool dst_vec = vec;
+    if (tl.ranges > 1) {
+        const int t = rho - tl.rho0;
+        const Partials part = partials(ws, a.n_kv, kv, gridDim.x / a.n_kv, w.item0 + w.range, kRowsPerWG, dim);
+        inv = 1.0f;
+        dst = part.o + t * dim;
+        dst_vec = false;
+        if (h == 0) {
+            part.ml[2 * t] = top;
+            part.ml[2 * t + 1] = l;
+        }
+    } else if (lse && h == 0) {
+        lse[(size_t)head * a.q_rows + sp.q0 + qi] = (top + log2f(l)) * kLn2;
+    }
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            floatx4 x;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = o[i][4 * u + e] * unit * inv;
+            store4(dst, 32 * i + 8 * u + 4 * h, dim, dst_vec, x);
+        }
+}
+
+// ---- backward --------------------------------------------------------------------------------
+
+// dq and d_i: tiles and lanes as in the forward pass; S^T = K Q^T, dP^T = V dO^T, dQ^T += K^T dS^T.
+template <int DP>
+__global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attn_split_dq_kernel(PackedAttn a, float* __restrict__ dq, float* __restrict__ delta,
+                                                               const float* __restrict__ dout, const float* __restrict__ out,
+                                                               const float* __restrict__ lse, const float* __restrict__ q,
+                                                               const float* __restrict__ k, const float* __restrict__ v) {
+    constexpr int KT = 32, U = DP / 8, NB = DP / 32;
+    __shared__ uintx4 kp[3 * KT * U];
+    __shared__ uintx4 vp[3 * KT * U];
+    const int kv = blockIdx.x % a.n_kv;
+    Work w;
+    if (!find_work<false, true>(a, kRowsPerWG, 0, blockIdx.x / a.n_kv, &w)) return;
+    const RowTile tl = row_tile(a, w, kRowsPerWG);
+    const Span sp = w.sp;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, c = lane & 31;
+    const int dim = a.head_dim, group = a.group, rows = tl.rows, shift = tl.shift, nkeys = tl.nkeys;
+    const bool vec = a.vec;
+    const int rho0 = tl.rho0 + wave * kRowsPerWave, rho = rho0 + c;
+    const bool live = rho < rows;
+    const int qi = (live ? rho : rows - 1) / group, head = kv * group + (live ? rho : rows - 1) % group;
+    const int limit = qi + shift;
+    const int first_limit = min(rho0, rows - 1) / group + shift;
+    const int last_limit = rho0 < rows ? (min(rho0 + kRowsPerWave, rows) - 1) / group + shift : -1;
+    const float* kb = k + (size_t)sp.k0 * a.k_rs + (size_t)kv * a.k_hs;
+    const float* vb = v + (size_t)sp.k0 * a.v_rs + (size_t)kv * a.v_hs;
+    const float* q_row = q + (size_t)(sp.q0 + qi) * a.q_rs + (size_t)head * dim;
+    const size_t o_at = (size_t)(sp.q0 + qi) * a.o_rs + (size_t)head * dim;
+    const float* g_row = dout + o_at;
+
+    Stage<KT, DP> ks, vs;
+    ks.load(kb, a.k_rs, 0, nkeys, dim, vec);
+    vs.load(vb, a.v_rs, 0, nkeys, dim, vec);
+    float d = 0.f;
+#pragma unroll
+    for (int st = 0; st < DP / 16; ++st)
+#pragma unroll
+        for (int e = 0; e < 8; e += 4) {
+            const floatx4 x = load4(g_row, 16 * st + 8 * h + e, dim, vec), y = load4(out + o_at, 16 * st + 8 * h + e, dim, vec);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) d += x[i] * y[i];
+        }
+    d += __shfl_xor(d, 32);
+    const size_t stat = (size_t)head * a.q_rows + sp.q0 + qi;
+    if (live && h == 0) delta[stat] = d;
+    const float lse2 = lse[stat] * kLog2e;
+    bf16x8 qp[3][DP / 16], gp[3][DP / 16];
+    load_operand<DP>(qp, q_row, h, dim, vec);
+    load_operand<DP>(gp, g_row, h, dim, vec);
+    floatx16 acc[NB];
+    clear(acc);
+    // Products s and dp over 32 keys at t0, in units 1 / u: the weights of the keys in dq / scale.
+    const float factor = a.scale * kLog2e;
+    auto weights = [&](const floatx16& s, floatx16 dp, int t0, float u) {
+        const bool edge = t0 + 31 > first_limit;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const float p = fast_exp2(fmaf(s[r], factor * u, -lse2)) * fmaf(dp[r], u, -d);
+            dp[r] = edge && t0 + acc_row(r, h) > limit ? 0.f : p;
+        }
+        return dp;
+    };
+    for (int t0 = 0; t0 < nkeys; t0 += KT) {
+        lds_barrier();
+        ks.store(kp);
+        vs.store(vp);
+        if (t0 + KT < nkeys) {
+            ks.load(kb, a.k_rs, t0 + KT, nkeys, dim, vec);
+            vs.load(vb, a.v_rs, t0 + KT, nkeys, dim, vec);
+        }
+        lds_barrier();
+        if (t0 > last_limit) continue;
+        const floatx16 s = tile_product<KT, DP>(kp, 0, qp, h, c);
+        const floatx16 dp = tile_product<KT, DP>(vp, 0, gp, h, c);
+        tile_add<KT, DP>(acc, kp, 0, weights(s, dp, t0, kDown2), lane);
+    }
+    float unit = kDown2;
+    if (any_not_finite(acc)) {
+        clear(acc);
+        unit = 1.0f;
+#pragma unroll 1
+        for (int t0 = 0; t0 < nkeys && t0 <= last_limit; t0 += 32) {
+            const size_t row = min(t0 + c, nkeys - 1);
+            const floatx16 s = rows_product<DP>(kb + row * a.k_rs, q_row, dim, vec, h);
+            const floatx16 ds = weights(s, rows_product<DP>(vb + row * a.v_rs, g_row, dim, vec, h), t0, 1.0f);
+            uint32_t seen = 0;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) seen |= (t0 + acc_row(r, h) <= min(limit, nkeys - 1) ? 1u : 0u) << r;
+            add_seen<DP>(acc, ds, seen, h, c, dim, vec, [&](int n) { return kb + (size_t)min(t0 + n, nkeys - 1) * a.k_rs; });
+        }
+    }
+    if (!live) return;
+    const float by = a.scale;
+    float* dst = dq + (size_t)(sp.q0 + qi) * a.q_rs + (size_t)head * dim;
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            floatx4 x;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = acc[i][4 * u + e] * unit * by;
+            store4(dst, 32 * i + 8 * u + 4 * h, dim, vec, x);
+        }
+}
+
+// dk and dv: a work-group per 128 keys of one (sequence, key head), a key per lane column with its K
+// and V parts in registers; the rows of the group's heads stream through LDS: S = Q K^T,
+// dP = dO V^T, dV^T += dO^T P, dK^T += Q^T dS.  Where there are few such tiles, their rows are cut into
+// gridDim.y parts (whole tiles of rows, of all heads in order); the parts' sums go to the workspace and
+// attn_split_dkv_join_kernel adds them in order.
+template <int DP>
+__global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attn_split_dkv_kernel(PackedAttn a, float* __restrict__ dk, float* __restrict__ dv,
+                                                                const float* __restrict__ delta, const float* __restrict__ dout,
+                                                                const float* __restrict__ lse, const float* __restrict__ q,
+                                                                const float* __restrict__ k, const float* __restrict__ v,
+                                                                float* __restrict__ part) {
+    constexpr int RT = 32, U = DP / 8, NB = DP / 32;
+    __shared__ uintx4 qp[3 * RT * U];
+    __shared__ uintx4 gp[3 * RT * U];
+    __shared__ __attribute__((aligned(16))) float stats[2][RT];
+    const int kv = blockIdx.x % a.n_kv;
+    Work w;
+    if (!find_work<true, true>(a, kRowsPerWG, 0, blockIdx.x / a.n_kv, &w)) return;
+    const Span sp = w.sp;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, c = lane & 31;
+    const int dim = a.head_dim, group = a.group;
+    const bool vec = a.vec;
+    const int key0 = w.tile * kRowsPerWG + wave * kRowsPerWave, key = key0 + c;
+    const bool live = key < (int)sp.kl;
+    const int shift = (int)sp.kl - (int)sp.ql, ql = sp.ql;
+    const size_t row = sp.k0 + (live ? key : (int)sp.kl - 1);
+    const float* k_row = k + row * a.k_rs + (size_t)kv * a.k_hs;
+    const float* v_row = v + row * a.v_rs + (size_t)kv * a.v_hs;
+    // The tiles of rows that see a key of the work-group, over the group's heads, and this part of them.
+    const int first = max(0, (int)w.tile * kRowsPerWG - shift) / RT, tiles = max(0, (ql + RT - 1) / RT - first);
+    const int64_t total = (int64_t)tiles * group;
+    const int it0 = (int)(total * blockIdx.y / gridDim.y), it1 = (int)(total * (blockIdx.y + 1) / gridDim.y);
+
+    bf16x8 kr[3][DP / 16], vr[3][DP / 16];
+    load_operand<DP>(kr, k_row, h, dim, vec);
+    load_operand<DP>(vr, v_row, h, dim, vec);
+    floatx16 ak[NB], av[NB];
+    clear(ak);
+    clear(av);
+    Stage<RT, DP> qs, gs;
+    float stat0 = 0.f, stat1 = 0.f;
+    auto load = [&](int it) {
+        const int head = kv * group + it / tiles, i0 = (first + it % tiles) * RT;
+        qs.load(q + (size_t)sp.q0 * a.q_rs + (size_t)head * dim, a.q_rs, i0, ql, dim, vec);
+        gs.load(dout + (size_t)sp.q0 * a.o_rs + (size_t)head * dim, a.o_rs, i0, ql, dim, vec);
+        if (threadIdx.x < RT) {
+            const size_t at = (size_t)head * a.q_rows + sp.q0 + min(i0 + (int)threadIdx.x, ql - 1);
+            const bool in = i0 + (int)threadIdx.x < ql;
+            stat0 = in ? lse[at] * kLog2e : 0.f;
+            stat1 = in ? delta[at] : 0.f;
+        }
+    };
+    const float factor = a.scale * kLog2e;
+    // From products s and dp (units 1 / u) of 32 rows at i0: p in s, ds / scale in dp.
+    auto weights = [&](floatx16& s, floatx16& dp, int i0, float u, const float* lse2, const float* d) {
+        const bool edge = key0 + kRowsPerWave - 1 > i0 + shift;
+#pragma unroll
+        for (int r = 0; r < 16; r += 4) {
+            const int i = acc_row(r, h);
+            const floatx4 m = *reinterpret_cast<const floatx4*>(lse2 + i), dd = *reinterpret_cast<const floatx4*>(d + i);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const bool off = edge && key > i0 + i + e + shift;
+                s[r + e] = off ? 0.f : fast_exp2(fmaf(s[r + e], factor * u, -m[e]));
+                dp[r + e] = off ? 0.f : s[r + e] * fmaf(dp[r + e], u, -dd[e]);
+            }
+        }
+    };
+    if (it0 < it1) load(it0);
+    for (int it = it0; it < it1; ++it) {
+        const int i0 = (first + it % tiles) * RT;
+        lds_barrier();
+        qs.store(qp);
+        gs.store(gp);
+        if (threadIdx.x < RT) {
+            stats[0][threadIdx.x] = stat0;
+            stats[1][threadIdx.x] = stat1;
+        }
+        if (it + 1 < it1) load(it + 1);
+        lds_barrier();
+        if (key0 > i0 + RT - 1 + shift) continue;  // no row of the tile sees a key of the wave
+        floatx16 s = tile_product<RT, DP>(qp, 0, kr, h, c);
+        floatx16 dp = tile_product<RT, DP>(gp, 0, vr, h, c);
+        weights(s, dp, i0, kDown2, stats[0], stats[1]);
+        tile_add<RT, DP>(av, gp, 0, s, lane);
+        tile_add<RT, DP>(ak, qp, 0, dp, lane);
+    }
+    float unit = kDown2;
+    if (any_not_finite(ak) || any_not_finite(av)) {
+        clear(ak);
+        clear(av);
+        unit = 1.0f;
+#pragma unroll 1
+        for (int it = it0; it < it1; ++it) {
+            const int head = kv * group + it / tiles, i0 = (first + it % tiles) * RT;
+            if (key0 > i0 + RT - 1 + shift) continue;
+            const float* qb = q + (size_t)sp.q0 * a.q_rs + (size_t)head * dim;
+            const float* gb = dout + (size_t)sp.q0 * a.o_rs + (size_t)head * dim;
+            const size_t at = (size_t)head * a.q_rows + sp.q0;
+            const size_t mine = min(i0 + c, ql - 1);
+            floatx16 s = rows_product<DP>(qb + mine * a.q_rs, k_row, dim, vec, h);
+            floatx16 dp = rows_product<DP>(gb + mine * a.o_rs, v_row, dim, vec, h);
+            uint32_t seen = 0;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int i = i0 + acc_row(r, h);
+                const bool on = i < ql && key <= i + shift;
+                seen |= (on ? 1u : 0u) << r;
+                s[r] = on ? fast_exp2(fmaf(s[r], factor, -lse[at + min(i, ql - 1)] * kLog2e)) : 0.f;
+                dp[r] = on ? s[r] * (dp[r] - delta[at + min(i, ql - 1)]) : 0.f;
+            }
+            add_seen<DP>(av, s, seen, h, c, dim, vec, [&](int n) { return gb + (size_t)min(i0 + n, ql - 1) * a.o_rs; });
+            add_seen<DP>(ak, dp, seen, h, c, dim, vec, [&](int n) { return qb + (size_t)min(i0 + n, ql - 1) * a.q_rs; });
+        }
+    }
+    if (!live) return;
+    float *dkr = dk + row * a.k_rs + (size_t)kv * a.k_hs, *dvr = dv + row * a.v_rs + (size_t)kv * a.v_hs;
+    bool dst_vec = vec;
+    if (gridDim.y > 1) {
+        const size_t tile = (size_t)blockIdx.y * gridDim.x + (size_t)w.tile0 * a.n_kv + kv;
+        dkr = part + (tile * 2 * kRowsPerWG + key - w.tile * kRowsPerWG) * DP;
+        dvr = dkr + kRowsPerWG * DP;
+        dst_vec = true;
+    }
+    const int width = gridDim.y > 1 ? DP : dim;
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int at = 32 * i + 8 * u + 4 * h;
+            floatx4 x, y;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                x[e] = ak[i][4 * u + e] * unit * a.scale;
+                y[e] = av[i][4 * u + e] * unit;
+            }
+            store4(dkr, at, width, dst_vec, x);
+            store4(dvr, at, width, dst_vec, y);
+        }
+}
+
+// dk and dv of a tile of keys: its parts added in order.
+template <int DP>
+__global__ __launch_bounds__(256) void attn_split_dkv_join_kernel(PackedAttn a, float* __restrict__ dk, float* __restrict__ dv,
+                                                                  const float* __restrict__ part, int parts) {
+    const int kv = blockIdx.x % a.n_kv;
+    Work w;
+    if (!find_work<true, true>(a, kRowsPerWG, 0, blockIdx.x / a.n_kv, &w)) return;
+    const int keys = min((int)w.sp.kl - (int)w.tile * kRowsPerWG, kRowsPerWG), dim = a.head_dim;
+    const size_t stride = (size_t)gridDim.x * 2 * kRowsPerWG * DP;
+    const float* p = part + ((size_t)w.tile0 * a.n_kv + kv) * 2 * kRowsPerWG * DP;
+    constexpr int N = 2 * kRowsPerWG * (DP / 4);
+    for (int e = blockIdx.y * 256 + threadIdx.x; e < N; e += 256 * gridDim.y) {
+        const int which = e / (N / 2), key = e % (N / 2) / (DP / 4), d = 4 * (e % (DP / 4));
+        if (key >= keys || d >= dim) continue;
+        floatx4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+        for (int z = 0; z < parts; ++z) x += *reinterpret_cast<const floatx4*>(p + z * stride + 4 * (size_t)e);
+        const size_t row = w.sp.k0 + (size_t)w.tile * kRowsPerWG + key;
+        store4(which ? dv + row * a.v_rs + (size_t)kv * a.v_hs : dk + row * a.k_rs + (size_t)kv * a.k_hs, d, dim, a.vec, x);
+    }
+}
+
+}  // namespace
+
+#define FMLH_BY_DIM(LAUNCH)                        \
+    do {                                           \
+        if (a.head_dim <= 32) LAUNCH(32);          \
+        else if (a.head_dim <= 64) LAUNCH(64);     \
+        else if (a.head_dim <= 96) LAUNCH(96);     \
+        else LAUNCH(128);                          \
+    } while (0)
+
+int attn_split_forward(const PackedAttn& a, uint32_t items, uint32_t budget, float* out, float* lse, const float* q, const float* k,
+                       const float* v, float* ws, hipStream_t s) {
+    const dim3 grid(items * a.n_kv);
+#define FMLH_LAUNCH(DP) hipLaunchKernelGGL(attn_split_kernel<DP>, grid, dim3(256), 0, s, a, out, lse, q, k, v, ws, budget)
+    FMLH_BY_DIM(FMLH_LAUNCH);
+#undef FMLH_LAUNCH
+    FMLH_LAUNCHED("attn_split_kernel");
+    return FMLH_OK;
+}
+
+int attn_split_dq(const PackedAttn& a, uint32_t tiles, float* dq, float* delta, const float* dout, const float* out, const float* lse,
+                  const float* q, const float* k, const float* v, hipStream_t s) {
+    const dim3 grid(tiles * a.n_kv);
+#define FMLH_LAUNCH(DP) hipLaunchKernelGGL(attn_split_dq_kernel<DP>, grid, dim3(256), 0, s, a, dq, delta, dout, out, lse, q, k, v)
+    FMLH_BY_DIM(FMLH_LAUNCH);
+#undef FMLH_LAUNCH
+    FMLH_LAUNCHED("attn_split_dq_kernel");
+    return FMLH_OK;
+}
+
+size_t attn_split_part_floats(const PackedAttn& a, uint32_t tiles) {
+    const size_t dp = a.head_dim <= 32 ? 32 : a.head_dim <= 64 ? 64 : a.head_dim <= 96 ? 96 : 128;
+    return (size_t)tiles * a.n_kv * 2 * kRowsPerWG * dp;
+}
+
+int attn_split_dkv(const PackedAttn& a, uint32_t tiles, int parts, float* dk, float* dv, const float* delta, const float* dout,
+                   const float* lse, const float* q, const float* k, const float* v, float* part, hipStream_t s) {
+    const dim3 grid(tiles * a.n_kv, parts);
+#define FMLH_LAUNCH(DP) \
+    hipLaunchKernelGGL(attn_split_dkv_kernel<DP>, grid, dim3(256), 0, s, a, dk, dv, delta, dout, lse, q, k, v, part)
+    FMLH_BY_DIM(FMLH_LAUNCH);
+#undef FMLH_LAUNCH
+    FMLH_LAUNCHED("attn_split_dkv_kernel");
+    if (parts > 1) {
+#define FMLH_LAUNCH(DP) hipLaunchKernelGGL(attn_split_dkv_join_kernel<DP>, dim3(grid.x, 8), dim3(256), 0, s, a, dk, dv, part, parts)
+        FMLH_BY_DIM(FMLH_LAUNCH);
+#undef FMLH_LAUNCH
+        FMLH_LAUNCHED("attn_split_dkv_join_kernel");
+    }
+    return FMLH_OK;
+}
+
+}  // namespace fmlh

@@ -6,8 +6,9 @@ a step of fp32 relative to the value).  A sum of n products in fp32 is off by at
 the sum of their absolute values.  With A the largest scale * sum |q| |k| of a row and D dims, a score
 is off by (D + 8) u A (product, scaling, the base-2 exponent's constant); a probability by ep =
 2 (D + 8) u A + (n + 8) u relative (numerator, and its share in the sum of n; exp2 is within two units),
-and out by sum p |v| (ep + n u).  lse, which the backward pass starts from, is off by (D + 8) u A + (n + 8) u
-and a rounding of its own size.  The gradients' bounds carry these on through their formulas.
+and out by sum p |v| (ep + n u).  A probability below 2^-126, fp32's smallest normal
+number, may come out as zero (the hardware's exponential gives no subnormal ones): 2^-126 more, absolute.
+lse, which the backward pass starts from, is off by (D + 8) u A + (n + 8) u and a rounding of its own size.  The gradients' bounds carry these on through their formulas.
 """
 import numpy as np
 import pytest
@@ -177,17 +178,19 @@ def reference(c, s, h, k=None, v=None):
     n = kl + 8
     ep = 2 * (D + 8) * U * A + n * U
     fin = np.where(np.isfinite(lse), np.abs(lse), 0.0)
-    b_out = p @ np.abs(v) * (ep + n * U)
+    low = np.where(seen, 2.0**-126, 0.0)  # of a probability that came out as zero
+    b_out = p @ np.abs(v) * (ep + n * U) + low @ np.abs(v)
     b_lse = ((D + 8) * U * A + n * U)[:, 0] + 2 * U * fin
     ep = ep + b_lse[:, None] + 4 * U * fin[:, None]  # p again, from lse
     dp, absdp = g @ v.T, np.abs(g) @ np.abs(v).T
     d, absd = (g * out).sum(1, keepdims=True), (np.abs(g) * np.abs(out)).sum(1, keepdims=True)
     ds = p * (dp - d) * scale
     b_ds = abs(scale) * p * (np.abs(dp - d) * (ep + 4 * U) + (absdp + absd) * (D + 8) * U + (np.abs(g) * b_out).sum(1, keepdims=True))
+    b_ds += abs(scale) * low * np.abs(dp - d)
     m = ql * G + 8
     return dict(out=out, lse=lse, q=ds @ k, k=ds.T @ q, v=p.T @ g, b_out=b_out, b_lse=b_lse,
                 b_q=b_ds @ np.abs(k) + np.abs(ds) @ np.abs(k) * n * U, b_k=b_ds.T @ np.abs(q) + np.abs(ds).T @ np.abs(q) * m * U,
-                b_v=(p * ep).T @ np.abs(g) + p.T @ np.abs(g) * m * U)
+                b_v=(p * ep + low).T @ np.abs(g) + p.T @ np.abs(g) * m * U)
 
 
 def close(got, ref, bound, what):
