@@ -30,6 +30,26 @@ __device__ __forceinline__ Span load_span(const PackedAttn& a, uint32_t s) {
     return p;
 }
 
+// Wave-wide integer sum and maximum (wave_reduce's lane shifts).
+template <class Op>
+__device__ __forceinline__ int wave_reduce_int(int v, int identity, Op op) {
+#define FMLH_STEP(CTRL, ROWS) v = op(v, __builtin_amdgcn_update_dpp(identity, v, CTRL, ROWS, 0xf, false))
+    FMLH_STEP(0x111, 0xf);
+    FMLH_STEP(0x112, 0xf);
+    FMLH_STEP(0x114, 0xf);
+    FMLH_STEP(0x118, 0xf);
+    FMLH_STEP(0x142, 0xa);
+    FMLH_STEP(0x143, 0xc);
+#undef FMLH_STEP
+    return __builtin_amdgcn_readlane(v, 63);
+}
+__device__ __forceinline__ int wave_sum_int(int v) {
+    return wave_reduce_int(v, 0, [](int a, int b) { return a + b; });
+}
+__device__ __forceinline__ int wave_max_int(int v) {
+    return wave_reduce_int(v, -0x7fffffff, [](int a, int b) { return max(a, b); });
+}
+
 // What a work-group does: tile `tile` of a sequence's `tiles`, and of the `ranges` that the sequence's
 // keys are cut into (`per` keys each) number `range`.  tile0 / item0: the tile's number, and that of
 // its first range, over all sequences.
@@ -47,6 +67,9 @@ constexpr int kRangeKeys = 128;  // a range is a multiple of this
 // keys of all tiles / budget, so that long sequences are cut and short ones are not (budget 0: none is).
 // Every wave scans the offsets, 64 sequences at a time.  False behind the last sequence: grids hold
 // sum / per_tile + n_seq tiles and budget items more, never fewer than there are.
+// Up to 64 sequences whose keys are not cut come in the order of their work, most first over all of
+// them: a tile's level falls by one from each to the next, and work number `index` lies on the highest
+// level T with more than index tiles on it and above.
 template <bool KEYS, bool BY_TILE>
 __device__ __forceinline__ bool find_work(const PackedAttn& a, uint32_t per_tile, uint32_t budget, uint32_t index, Work* w) {
     const uint32_t lane = threadIdx.x & 63;
@@ -66,6 +89,40 @@ __device__ __forceinline__ bool find_work(const PackedAttn& a, uint32_t per_tile
         for (int d = 32; d >= 1; d >>= 1) keys += __shfl_xor((unsigned long long)keys, d);
         const uint64_t per = (keys / budget + kRangeKeys) / kRangeKeys * kRangeKeys;
         w->per = (int)min(per, (uint64_t)0x40000000);
+    }
+    if (!budget && a.n_seq <= 64) {
+        if (lane < a.n_seq) p = load_span(a, lane);
+        const int n = tiles_of(p);  // at most 2^23, and a level 2^24: sums over 64 lanes stay inside 32 bits
+        // Keys that a sequence's last tile sees (rows that see its first tile), in tiles.
+        const int top = (int)min(KEYS ? (uint64_t)p.ql / per_tile : (uint64_t)p.kl * a.group / per_tile, (uint64_t)1 << 24);
+        auto above = [&](int T) { return (uint32_t)wave_sum_int(min(max(top - T + 1, 0), n)); };  // tiles of level T and more
+        int lo = -wave_max_int(n - top), hi = wave_max_int(top) + 1;  // above(lo) holds all, above(hi) none
+        if (above(lo) <= index) return false;
+        while (hi - lo > 1) {
+            const int mid = lo + (hi - lo) / 2;
+            if (above(mid) > index) lo = mid;
+            else hi = mid;
+        }
+        const bool on = top - lo >= 0 && top - lo < n;
+        const uint64_t level = __ballot(on);
+        const uint32_t r = index - above(hi), mine = __builtin_popcountll(level & ((1ull << lane) - 1));
+        const int l = __builtin_ctzll(__ballot(on && mine == r));
+        uint32_t upto = n;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const uint32_t x = __shfl_up(upto, d);
+            if (lane >= (uint32_t)d) upto += x;
+        }
+        w->sp.q0 = __shfl(p.q0, l);
+        w->sp.ql = __shfl(p.ql, l);
+        w->sp.k0 = __shfl(p.k0, l);
+        w->sp.kl = __shfl(p.kl, l);
+        w->tiles = __shfl(n, l);
+        w->tile = __shfl(KEYS ? top - lo : n - 1 - (top - lo), l);
+        w->tile0 = w->item0 = __shfl(upto - n, l) + w->tile;
+        w->range = 0;
+        w->ranges = 1;
+        return true;
     }
     uint32_t tiles_before = 0, items_before = 0;
     for (uint32_t base = 0; base < a.n_seq; base += 64) {
@@ -146,6 +203,26 @@ __device__ __forceinline__ floatx4 load4(const float* row, int d, int dim, bool 
             if (d + e < dim) v[e] = row[d + e];
     }
     return v;
+}
+
+// Dims d .. d + 3 where at least d + 3 < DP; VEC: from memory without a branch, whatever lies past
+// head_dim replaced by zeros.
+template <bool VEC>
+__device__ __forceinline__ floatx4 load4_padded(const float* row, int d, int dim, bool on) {
+    if constexpr (VEC) {
+        const bool in = on && d < dim;
+        const floatx4 x = *reinterpret_cast<const floatx4*>(row + (in ? d : 0));
+        floatx4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = in ? x[e] : 0.f;
+        return v;
+    } else {
+        floatx4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (on && d + e < dim) v[e] = row[d + e];
+        return v;
+    }
 }
 
 __device__ __forceinline__ void store4(float* row, int d, int dim, bool vec, floatx4 v) {

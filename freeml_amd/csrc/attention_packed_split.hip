@@ -32,28 +32,38 @@ struct Shape {
     __device__ static __forceinline__ int swz(int r) { return U % 8 == 0 ? (r & 7) : ((r >> 2) & 3); }
 };
 
-// R rows of a matrix in registers (a thread's share) and from there as planes in LDS.
-template <int R, int DP>
+// R rows of a matrix in the registers of 256 threads (a thread's share) and from there as planes in LDS.
+template <int R, int DP, bool VEC>
 struct Stage {
     static constexpr int U = DP / 8, N = (R * U + 255) / 256;
     floatx4 x[N][2];
-    // Rows first .. of a matrix at base, row stride rs; rows from `rows` on are zeros.
-    __device__ __forceinline__ void load(const float* base, size_t rs, int first, int rows, int dim, bool vec) {
+    // Rows first .. of a matrix at base (64-bit, uniform), row stride rs; rows from `rows` on (rows > first) are zeros.
+    __device__ __forceinline__ void load(const float* base, size_t rs, int first, int rows, int dim) {
+        const int t = threadIdx.x & 255;
+        const float* tile = base + (size_t)first * rs;
+        if (VEC && R * U % 256 == 0 && first + R <= rows && dim == DP) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int u = t + 256 * i;
+                const floatx4* row = reinterpret_cast<const floatx4*>(tile + (size_t)(u / U) * rs + 8 * (u % U));
+                x[i][0] = row[0];
+                x[i][1] = row[1];
+            }
+            return;
+        }
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int u = threadIdx.x + 256 * i, r = first + u / U, d = 8 * (u % U);
-            x[i][0] = x[i][1] = floatx4{0.f, 0.f, 0.f, 0.f};
-            if (r < rows && (R * U % 256 == 0 || u < R * U)) {
-                const float* row = base + (size_t)r * rs;
-                x[i][0] = load4(row, d, dim, vec);
-                x[i][1] = load4(row, d + 4, dim, vec);
-            }
+            const int u = min(t + 256 * i, R * U - 1), r = u / U, d = 8 * (u % U);
+            const bool on = first + r < rows;
+            const float* row = tile + (size_t)(on ? r : 0) * rs;
+            x[i][0] = load4_padded<VEC>(row, d, dim, on);
+            x[i][1] = load4_padded<VEC>(row, d + 4, dim, on);
         }
     }
     __device__ __forceinline__ void store(uintx4* planes) const {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int u = threadIdx.x + 256 * i, r = u / U;
+            const int u = (threadIdx.x & 255) + 256 * i, r = u / U;
             if (R * U % 256 != 0 && u >= R * U) break;
             const float v[8] = {x[i][0][0], x[i][0][1], x[i][0][2], x[i][0][3], x[i][1][0], x[i][1][1], x[i][1][2], x[i][1][3]};
             uintx4 p[3];
@@ -89,11 +99,11 @@ __device__ __forceinline__ bf16x8 column_operand(const uintx4* planes, int q, in
 }
 
 // A lane's row as operand of products over the dims: dims 16 st + 8 h .. of every step, three parts.
-template <int DP>
-__device__ __forceinline__ void load_operand(bf16x8 (&p)[3][DP / 16], const float* row, int h, int dim, bool vec) {
+template <int DP, bool VEC>
+__device__ __forceinline__ void load_operand(bf16x8 (&p)[3][DP / 16], const float* row, int h, int dim) {
 #pragma unroll
     for (int st = 0; st < DP / 16; ++st) {
-        const floatx4 a = load4(row, 16 * st + 8 * h, dim, vec), b = load4(row, 16 * st + 8 * h + 4, dim, vec);
+        const floatx4 a = load4_padded<VEC>(row, 16 * st + 8 * h, dim, true), b = load4_padded<VEC>(row, 16 * st + 8 * h + 4, dim, true);
         const float v[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
         uintx4 u[3];
         split8(v, u, kUp);
@@ -159,7 +169,55 @@ __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_ex
 
 // ---- forward ---------------------------------------------------------------------------------
 
+// Output, maximum and sum of 32 rows again, from memory (a wave whose results are not finite).
 template <int DP>
+struct Redone {
+    floatx16 x[DP / 32];
+    float top, l;
+};
+template <int DP>
+__device__ __noinline__ void redo_rows(Redone<DP>& result, const PackedAttn& a, const float* kb, const float* vb, const float* q_row,
+                                       int k_begin, int k_end, int limit, int last_limit) {
+    const int lane = threadIdx.x & 63, h = lane >> 5, c = lane & 31;
+    const float factor = a.scale * kLog2e;
+    floatx16 o[DP / 32];
+    clear(o);
+    float top = -INFINITY, l = 0.f;
+#pragma unroll 1
+    for (int t0 = k_begin; t0 < k_end && t0 <= last_limit; t0 += 32) {
+        floatx16 s = rows_product<DP>(kb + (size_t)min(t0 + c, k_end - 1) * a.k_rs, q_row, a.head_dim, a.vec, h);
+        uint32_t seen = 0;
+        float mt = top;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const bool on = t0 + acc_row(r, h) <= limit;
+            seen |= (on ? 1u : 0u) << r;
+            s[r] = on ? s[r] * factor : -INFINITY;
+            mt = fmaxf(mt, s[r]);
+        }
+        mt = fmaxf(mt, __shfl_xor(mt, 32));
+        const float base = mt == -INFINITY ? 0.f : mt, corr = fast_exp2(top - base);
+        top = mt;
+        float sum = 0.f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            s[r] = fast_exp2(s[r] - base);
+            sum += s[r];
+        }
+        l = l * corr + sum;
+#pragma unroll
+        for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) o[i][r] *= corr;
+        add_seen<DP>(o, s, seen, h, c, a.head_dim, a.vec, [&](int n) { return vb + (size_t)min(t0 + n, k_end - 1) * a.v_rs; });
+    }
+#pragma unroll
+    for (int i = 0; i < DP / 32; ++i) result.x[i] = o[i];
+    result.top = top;
+    result.l = l;
+}
+
+template <int DP, bool VEC>
 __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attn_split_kernel(PackedAttn a, float* __restrict__ out, float* __restrict__ lse,
                                                             const float* __restrict__ q, const float* __restrict__ k,
                                                             const float* __restrict__ v, float* __restrict__ ws, uint32_t budget) {
@@ -187,11 +245,13 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attn_split_kernel(Packe
     const float* vb = v + (size_t)sp.k0 * a.v_rs + (size_t)kv * a.v_hs;
     const float* q_row = q + (size_t)(sp.q0 + qi) * a.q_rs + (size_t)head * dim;
 
-    Stage<KT, DP> ks, vs;
-    ks.load(kb, a.k_rs, k_begin, k_end, dim, vec);
-    vs.load(vb, a.v_rs, k_begin, k_end, dim, vec);
+    Stage<KT, DP, VEC> ks, vs;
+    if (k_begin < k_end) {
+        ks.load(kb, a.k_rs, k_begin, k_end, dim);
+        vs.load(vb, a.v_rs, k_begin, k_end, dim);
+    }
     bf16x8 qp[3][DP / 16];
-    load_operand<DP>(qp, q_row, h, dim, vec);
+    load_operand<DP, VEC>(qp, q_row, h, dim);
     floatx16 o[NB];
     clear(o);
     float top = -INFINITY, l = 0.f;  // the running maximum of the raw products, the sum of exponentials
@@ -232,8 +292,8 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attn_split_kernel(Packe
         ks.store(kp);
         vs.store(vp);
         if (t0 + KT < k_end) {
-            ks.load(kb, a.k_rs, t0 + KT, k_end, dim, vec);
-            vs.load(vb, a.v_rs, t0 + KT, k_end, dim, vec);
+            ks.load(kb, a.k_rs, t0 + KT, k_end, dim);
+            vs.load(vb, a.v_rs, t0 + KT, k_end, dim);
         }
         lds_barrier();
         if (t0 > last_limit) continue;  // no row of the wave sees the tile
@@ -246,21 +306,13 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attn_split_kernel(Packe
     }
     float unit = kDown2;
     if (any_not_finite(o)) {
-        clear(o);
-        top = -INFINITY;
-        l = 0.f;
         unit = 1.0f;
-#pragma unroll 1
-        for (int t0 = k_begin; t0 < k_end && t0 <= last_limit; t0 += 32) {
-            const int lk = k_end - 1;
-            floatx16 s[1];
-            s[0] = rows_product<DP>(kb + (size_t)min(t0 + c, lk) * a.k_rs, q_row, dim, vec, h);
-            softmax(s, 1, t0, factor);
-            uint32_t seen = 0;
+        Redone<DP> r;  // a copy: o itself stays in registers
+        redo_rows<DP>(r, a, kb, vb, q_row, k_begin, k_end, limit, last_limit);
 #pragma unroll
-            for (int r = 0; r < 16; ++r) seen |= (t0 + acc_row(r, h) <= limit ? 1u : 0u) << r;
-            add_seen<DP>(o, s[0], seen, h, c, dim, vec, [&](int n) { return vb + (size_t)min(t0 + n, lk) * a.v_rs; });
-        }
+        for (int i = 0; i < NB; ++i) o[i] = r.x[i];
+        top = r.top;
+        l = r.l;
     }
     l += __shfl_xor(l, 32);
     if (!live) return;
@@ -294,7 +346,32 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attn_split_kernel(Packe
 // ---- backward --------------------------------------------------------------------------------
 
 // dq and d_i: tiles and lanes as in the forward pass; S^T = K Q^T, dP^T = V dO^T, dQ^T += K^T dS^T.
+// dq / scale of 32 rows again, from memory.
 template <int DP>
+__device__ __noinline__ void redo_dq(Redone<DP>& result, const PackedAttn& a, const float* kb, const float* vb, const float* q_row,
+                                     const float* g_row, float lse2, float d, int nkeys, int limit, int last_limit) {
+    const int lane = threadIdx.x & 63, h = lane >> 5, c = lane & 31;
+    floatx16 acc[DP / 32];
+    clear(acc);
+#pragma unroll 1
+    for (int t0 = 0; t0 < nkeys && t0 <= last_limit; t0 += 32) {
+        const size_t row = min(t0 + c, nkeys - 1);
+        floatx16 s = rows_product<DP>(kb + row * a.k_rs, q_row, a.head_dim, a.vec, h);
+        const floatx16 dp = rows_product<DP>(vb + row * a.v_rs, g_row, a.head_dim, a.vec, h);
+        uint32_t seen = 0;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const bool on = t0 + acc_row(r, h) <= min(limit, nkeys - 1);
+            seen |= (on ? 1u : 0u) << r;
+            s[r] = on ? fast_exp2(fmaf(s[r], a.scale * kLog2e, -lse2)) * (dp[r] - d) : 0.f;
+        }
+        add_seen<DP>(acc, s, seen, h, c, a.head_dim, a.vec, [&](int n) { return kb + (size_t)min(t0 + n, nkeys - 1) * a.k_rs; });
+    }
+#pragma unroll
+    for (int i = 0; i < DP / 32; ++i) result.x[i] = acc[i];
+}
+
+template <int DP, bool VEC>
 __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attn_split_dq_kernel(PackedAttn a, float* __restrict__ dq, float* __restrict__ delta,
                                                                const float* __restrict__ dout, const float* __restrict__ out,
                                                                const float* __restrict__ lse, const float* __restrict__ q,
@@ -322,15 +399,18 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attn_split_dq_kernel(Pa
     const size_t o_at = (size_t)(sp.q0 + qi) * a.o_rs + (size_t)head * dim;
     const float* g_row = dout + o_at;
 
-    Stage<KT, DP> ks, vs;
-    ks.load(kb, a.k_rs, 0, nkeys, dim, vec);
-    vs.load(vb, a.v_rs, 0, nkeys, dim, vec);
+    Stage<KT, DP, VEC> ks, vs;
+    if (nkeys > 0) {
+        ks.load(kb, a.k_rs, 0, nkeys, dim);
+        vs.load(vb, a.v_rs, 0, nkeys, dim);
+    }
     float d = 0.f;
 #pragma unroll
     for (int st = 0; st < DP / 16; ++st)
 #pragma unroll
         for (int e = 0; e < 8; e += 4) {
-            const floatx4 x = load4(g_row, 16 * st + 8 * h + e, dim, vec), y = load4(out + o_at, 16 * st + 8 * h + e, dim, vec);
+            const floatx4 x = load4_padded<VEC>(g_row, 16 * st + 8 * h + e, dim, true),
+                          y = load4_padded<VEC>(out + o_at, 16 * st + 8 * h + e, dim, true);
 #pragma unroll
             for (int i = 0; i < 4; ++i) d += x[i] * y[i];
         }
@@ -339,49 +419,38 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attn_split_dq_kernel(Pa
     if (live && h == 0) delta[stat] = d;
     const float lse2 = lse[stat] * kLog2e;
     bf16x8 qp[3][DP / 16], gp[3][DP / 16];
-    load_operand<DP>(qp, q_row, h, dim, vec);
-    load_operand<DP>(gp, g_row, h, dim, vec);
+    load_operand<DP, VEC>(qp, q_row, h, dim);
+    load_operand<DP, VEC>(gp, g_row, h, dim);
     floatx16 acc[NB];
     clear(acc);
-    // Products s and dp over 32 keys at t0, in units 1 / u: the weights of the keys in dq / scale.
     const float factor = a.scale * kLog2e;
-    auto weights = [&](const floatx16& s, floatx16 dp, int t0, float u) {
-        const bool edge = t0 + 31 > first_limit;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            const float p = fast_exp2(fmaf(s[r], factor * u, -lse2)) * fmaf(dp[r], u, -d);
-            dp[r] = edge && t0 + acc_row(r, h) > limit ? 0.f : p;
-        }
-        return dp;
-    };
     for (int t0 = 0; t0 < nkeys; t0 += KT) {
         lds_barrier();
         ks.store(kp);
         vs.store(vp);
         if (t0 + KT < nkeys) {
-            ks.load(kb, a.k_rs, t0 + KT, nkeys, dim, vec);
-            vs.load(vb, a.v_rs, t0 + KT, nkeys, dim, vec);
+            ks.load(kb, a.k_rs, t0 + KT, nkeys, dim);
+            vs.load(vb, a.v_rs, t0 + KT, nkeys, dim);
         }
         lds_barrier();
         if (t0 > last_limit) continue;
-        const floatx16 s = tile_product<KT, DP>(kp, 0, qp, h, c);
+        floatx16 s = tile_product<KT, DP>(kp, 0, qp, h, c);
         const floatx16 dp = tile_product<KT, DP>(vp, 0, gp, h, c);
-        tile_add<KT, DP>(acc, kp, 0, weights(s, dp, t0, kDown2), lane);
+        const bool edge = t0 + 31 > first_limit;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const float x = fast_exp2(fmaf(s[r], factor * kDown2, -lse2)) * fmaf(dp[r], kDown2, -d);
+            s[r] = edge && t0 + acc_row(r, h) > limit ? 0.f : x;
+        }
+        tile_add<KT, DP>(acc, kp, 0, s, lane);
     }
     float unit = kDown2;
     if (any_not_finite(acc)) {
-        clear(acc);
         unit = 1.0f;
-#pragma unroll 1
-        for (int t0 = 0; t0 < nkeys && t0 <= last_limit; t0 += 32) {
-            const size_t row = min(t0 + c, nkeys - 1);
-            const floatx16 s = rows_product<DP>(kb + row * a.k_rs, q_row, dim, vec, h);
-            const floatx16 ds = weights(s, rows_product<DP>(vb + row * a.v_rs, g_row, dim, vec, h), t0, 1.0f);
-            uint32_t seen = 0;
+        Redone<DP> r;
+        redo_dq<DP>(r, a, kb, vb, q_row, g_row, lse2, d, nkeys, limit, last_limit);
 #pragma unroll
-            for (int r = 0; r < 16; ++r) seen |= (t0 + acc_row(r, h) <= min(limit, nkeys - 1) ? 1u : 0u) << r;
-            add_seen<DP>(acc, ds, seen, h, c, dim, vec, [&](int n) { return kb + (size_t)min(t0 + n, nkeys - 1) * a.k_rs; });
-        }
+        for (int i = 0; i < NB; ++i) acc[i] = r.x[i];
     }
     if (!live) return;
     const float by = a.scale;
@@ -397,29 +466,84 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attn_split_dq_kernel(Pa
         }
 }
 
-// dk and dv: a work-group per 128 keys of one (sequence, key head), a key per lane column with its K
-// and V parts in registers; the rows of the group's heads stream through LDS: S = Q K^T,
-// dP = dO V^T, dV^T += dO^T P, dK^T += Q^T dS.  Where there are few such tiles, their rows are cut into
-// gridDim.y parts (whole tiles of rows, of all heads in order); the parts' sums go to the workspace and
-// attn_split_dkv_join_kernel adds them in order.
+// The two waves of a pair hand 32 x 32 values to one another through LDS as their accumulators lie.
+struct Exchange {
+    floatx4 x[4][64];
+    __device__ __forceinline__ void put(const floatx16& v, int lane) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) x[u][lane] = floatx4{v[4 * u], v[4 * u + 1], v[4 * u + 2], v[4 * u + 3]};
+    }
+    __device__ __forceinline__ floatx16 get(int lane) const {
+        floatx16 v;
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[4 * u + e] = x[u][lane][e];
+        return v;
+    }
+};
+
+// The sums of 32 keys again, from memory (a wave whose results are not finite).
 template <int DP>
-__global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attn_split_dkv_kernel(PackedAttn a, float* __restrict__ dk, float* __restrict__ dv,
+__device__ __noinline__ void redo_dkv(Redone<DP>& result, const PackedAttn& a, const Span& sp, int kv, int second, int key0,
+                                         int first, int tiles, int it0, int it1, int rt, const float* delta, const float* dout,
+                                         const float* lse, const float* q, const float* k_row, const float* v_row) {
+    const int lane = threadIdx.x & 63, h = lane >> 5, c = lane & 31, ql = sp.ql, shift = (int)sp.kl - (int)sp.ql;
+    floatx16 acc[DP / 32];
+    clear(acc);
+#pragma unroll 1
+    for (int block = it0 * (rt / 32); block < it1 * (rt / 32); ++block) {
+        const int it = block / (rt / 32), head = kv * a.group + it / tiles, i0 = (first + it % tiles) * rt + 32 * (block % (rt / 32));
+        if (key0 > i0 + 31 + shift || i0 >= ql) continue;
+        const float* qb = q + (size_t)sp.q0 * a.q_rs + (size_t)head * a.head_dim;
+        const float* gb = dout + (size_t)sp.q0 * a.o_rs + (size_t)head * a.head_dim;
+        const size_t at = (size_t)head * a.q_rows + sp.q0;
+        const size_t mine = min(i0 + c, ql - 1);
+        floatx16 s = rows_product<DP>(qb + mine * a.q_rs, k_row, a.head_dim, a.vec, h);
+        const floatx16 dp = rows_product<DP>(gb + mine * a.o_rs, v_row, a.head_dim, a.vec, h);
+        uint32_t seen = 0;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const int i = i0 + acc_row(r, h), j = min(i, ql - 1);
+            const bool on = i < ql && key0 + c <= i + shift;
+            seen |= (on ? 1u : 0u) << r;
+            const float p = fast_exp2(fmaf(s[r], a.scale * kLog2e, -lse[at + j] * kLog2e));
+            s[r] = on ? (second ? p * (dp[r] - delta[at + j]) : p) : 0.f;
+        }
+        const float* base = second ? qb : gb;
+        const size_t rs = second ? a.q_rs : a.o_rs;
+        add_seen<DP>(acc, s, seen, h, c, a.head_dim, a.vec, [&](int n) { return base + (size_t)min(i0 + n, ql - 1) * rs; });
+    }
+#pragma unroll
+    for (int i = 0; i < DP / 32; ++i) result.x[i] = acc[i];
+}
+
+// dk and dv: a work-group per 128 keys of one (sequence, key head), a key per lane column; the rows of
+// the group's heads stream through LDS.  Two waves share 32 keys (keeping K and V parts and both sums
+// in one wave's registers spilled at head_dim 128: 4.9 ms where this takes @DKV128@):
+//   the first   S = Q K^T, p, dV^T += dO^T P     holds K and dV,
+//   the second  dP = dO V^T, dS, dK^T += Q^T dS  holds V and dK and takes p from the first.
+// Where there are few such tiles, their rows are cut into gridDim.y parts (whole tiles of rows, of
+// all heads in order); the parts' sums go to the workspace and attn_split_dkv_join_kernel adds them in order.
+template <int DP, bool VEC>
+__global__ __launch_bounds__(512, DP == 32 ? 4 : 2) void attn_split_dkv_kernel(PackedAttn a, float* __restrict__ dk, float* __restrict__ dv,
                                                                 const float* __restrict__ delta, const float* __restrict__ dout,
                                                                 const float* __restrict__ lse, const float* __restrict__ q,
                                                                 const float* __restrict__ k, const float* __restrict__ v,
                                                                 float* __restrict__ part) {
-    constexpr int RT = 32, U = DP / 8, NB = DP / 32;
-    __shared__ uintx4 qp[3 * RT * U];
-    __shared__ uintx4 gp[3 * RT * U];
-    __shared__ __attribute__((aligned(16))) float stats[2][RT];
+    constexpr int RT = DP == 64 ? 64 : 32, U = DP / 8, NB = DP / 32;
+    __shared__ uintx4 planes[2][3 * RT * U];  // Q, dO
+    __shared__ Exchange exchange[RT / 32][4];
+    __shared__ __attribute__((aligned(16))) float stats[2][RT];  // lse (base 2), d
     const int kv = blockIdx.x % a.n_kv;
     Work w;
     if (!find_work<true, true>(a, kRowsPerWG, 0, blockIdx.x / a.n_kv, &w)) return;
     const Span sp = w.sp;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, c = lane & 31;
+    const int pair = wave & 3, second = wave >> 2;
     const int dim = a.head_dim, group = a.group;
     const bool vec = a.vec;
-    const int key0 = w.tile * kRowsPerWG + wave * kRowsPerWave, key = key0 + c;
+    const int key0 = w.tile * kRowsPerWG + pair * kRowsPerWave, key = key0 + c;
     const bool live = key < (int)sp.kl;
     const int shift = (int)sp.kl - (int)sp.ql, ql = sp.ql;
     const size_t row = sp.k0 + (live ? key : (int)sp.kl - 1);
@@ -430,111 +554,99 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attn_split_dkv_kernel(P
     const int64_t total = (int64_t)tiles * group;
     const int it0 = (int)(total * blockIdx.y / gridDim.y), it1 = (int)(total * (blockIdx.y + 1) / gridDim.y);
 
-    bf16x8 kr[3][DP / 16], vr[3][DP / 16];
-    load_operand<DP>(kr, k_row, h, dim, vec);
-    load_operand<DP>(vr, v_row, h, dim, vec);
-    floatx16 ak[NB], av[NB];
-    clear(ak);
-    clear(av);
-    Stage<RT, DP> qs, gs;
-    float stat0 = 0.f, stat1 = 0.f;
+    bf16x8 own[3][DP / 16];  // K's, V's parts
+    load_operand<DP, VEC>(own, second ? v_row : k_row, h, dim);
+    floatx16 acc[NB];  // dV^T, dK^T
+    clear(acc);
+    // The first four waves stage Q and lse, the others dO and d.
+    Stage<RT, DP, VEC> rows;
+    float stat = 0.f;
+    const float* const rows_base = second ? dout + (size_t)sp.q0 * a.o_rs : q + (size_t)sp.q0 * a.q_rs;
+    const float* const stat_base = second ? delta : lse;
+    const size_t rows_rs = second ? a.o_rs : a.q_rs;
     auto load = [&](int it) {
         const int head = kv * group + it / tiles, i0 = (first + it % tiles) * RT;
-        qs.load(q + (size_t)sp.q0 * a.q_rs + (size_t)head * dim, a.q_rs, i0, ql, dim, vec);
-        gs.load(dout + (size_t)sp.q0 * a.o_rs + (size_t)head * dim, a.o_rs, i0, ql, dim, vec);
-        if (threadIdx.x < RT) {
-            const size_t at = (size_t)head * a.q_rows + sp.q0 + min(i0 + (int)threadIdx.x, ql - 1);
-            const bool in = i0 + (int)threadIdx.x < ql;
-            stat0 = in ? lse[at] * kLog2e : 0.f;
-            stat1 = in ? delta[at] : 0.f;
-        }
+        rows.load(rows_base + (size_t)head * dim, rows_rs, i0, ql, dim);
+        const int i = i0 + (threadIdx.x & 255);
+        if ((threadIdx.x & 255) < RT) stat = i < ql ? stat_base[(size_t)head * a.q_rows + sp.q0 + i] * (second ? 1.0f : kLog2e) : 0.f;
     };
     const float factor = a.scale * kLog2e;
-    // From products s and dp (units 1 / u) of 32 rows at i0: p in s, ds / scale in dp.
-    auto weights = [&](floatx16& s, floatx16& dp, int i0, float u, const float* lse2, const float* d) {
-        const bool edge = key0 + kRowsPerWave - 1 > i0 + shift;
-#pragma unroll
-        for (int r = 0; r < 16; r += 4) {
-            const int i = acc_row(r, h);
-            const floatx4 m = *reinterpret_cast<const floatx4*>(lse2 + i), dd = *reinterpret_cast<const floatx4*>(d + i);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const bool off = edge && key > i0 + i + e + shift;
-                s[r + e] = off ? 0.f : fast_exp2(fmaf(s[r + e], factor * u, -m[e]));
-                dp[r + e] = off ? 0.f : s[r + e] * fmaf(dp[r + e], u, -dd[e]);
-            }
-        }
-    };
     if (it0 < it1) load(it0);
     for (int it = it0; it < it1; ++it) {
         const int i0 = (first + it % tiles) * RT;
         lds_barrier();
-        qs.store(qp);
-        gs.store(gp);
-        if (threadIdx.x < RT) {
-            stats[0][threadIdx.x] = stat0;
-            stats[1][threadIdx.x] = stat1;
-        }
+        rows.store(planes[second]);
+        if ((threadIdx.x & 255) < RT) stats[second][threadIdx.x & 255] = stat;
         if (it + 1 < it1) load(it + 1);
         lds_barrier();
-        if (key0 > i0 + RT - 1 + shift) continue;  // no row of the tile sees a key of the wave
-        floatx16 s = tile_product<RT, DP>(qp, 0, kr, h, c);
-        floatx16 dp = tile_product<RT, DP>(gp, 0, vr, h, c);
-        weights(s, dp, i0, kDown2, stats[0], stats[1]);
-        tile_add<RT, DP>(av, gp, 0, s, lane);
-        tile_add<RT, DP>(ak, qp, 0, dp, lane);
-    }
-    float unit = kDown2;
-    if (any_not_finite(ak) || any_not_finite(av)) {
-        clear(ak);
-        clear(av);
-        unit = 1.0f;
-#pragma unroll 1
-        for (int it = it0; it < it1; ++it) {
-            const int head = kv * group + it / tiles, i0 = (first + it % tiles) * RT;
-            if (key0 > i0 + RT - 1 + shift) continue;
-            const float* qb = q + (size_t)sp.q0 * a.q_rs + (size_t)head * dim;
-            const float* gb = dout + (size_t)sp.q0 * a.o_rs + (size_t)head * dim;
-            const size_t at = (size_t)head * a.q_rows + sp.q0;
-            const size_t mine = min(i0 + c, ql - 1);
-            floatx16 s = rows_product<DP>(qb + mine * a.q_rs, k_row, dim, vec, h);
-            floatx16 dp = rows_product<DP>(gb + mine * a.o_rs, v_row, dim, vec, h);
-            uint32_t seen = 0;
+        floatx16 s[RT / 32];
+        // Blocks of 32 rows: none of a block's rows may see the wave's keys, or not all of them all.
+        auto needed = [&](int j) { return key0 <= i0 + 32 * j + 31 + shift; };
+        auto hidden = [&](int j, int r) { return key > i0 + 32 * j + r + shift; };
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int i = i0 + acc_row(r, h);
-                const bool on = i < ql && key <= i + shift;
-                seen |= (on ? 1u : 0u) << r;
-                s[r] = on ? fast_exp2(fmaf(s[r], factor, -lse[at + min(i, ql - 1)] * kLog2e)) : 0.f;
-                dp[r] = on ? s[r] * (dp[r] - delta[at + min(i, ql - 1)]) : 0.f;
+        for (int j = 0; j < RT / 32; ++j) {
+            if (!needed(j)) continue;
+            s[j] = tile_product<RT, DP>(planes[second], 32 * j, own, h, c);
+            if (second) continue;
+            const bool edge = key0 + kRowsPerWave - 1 > i0 + 32 * j + shift;
+#pragma unroll
+            for (int r = 0; r < 16; r += 4) {
+                const floatx4 m = *reinterpret_cast<const floatx4*>(&stats[0][32 * j + acc_row(r, h)]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float p = fast_exp2(fmaf(s[j][r + e], factor * kDown2, -m[e]));
+                    s[j][r + e] = edge && hidden(j, acc_row(r, h) + e) ? 0.f : p;
+                }
             }
-            add_seen<DP>(av, s, seen, h, c, dim, vec, [&](int n) { return gb + (size_t)min(i0 + n, ql - 1) * a.o_rs; });
-            add_seen<DP>(ak, dp, seen, h, c, dim, vec, [&](int n) { return qb + (size_t)min(i0 + n, ql - 1) * a.q_rs; });
+            exchange[j][pair].put(s[j], lane);
+        }
+        lds_barrier();
+#pragma unroll
+        for (int j = 0; j < RT / 32; ++j) {
+            if (!needed(j)) continue;
+            if (second) {
+                const floatx16 p = exchange[j][pair].get(lane);
+                const bool edge = key0 + kRowsPerWave - 1 > i0 + 32 * j + shift;
+#pragma unroll
+                for (int r = 0; r < 16; r += 4) {
+                    const floatx4 d = *reinterpret_cast<const floatx4*>(&stats[1][32 * j + acc_row(r, h)]);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float x = p[r + e] * fmaf(s[j][r + e], kDown2, -d[e]);
+                        s[j][r + e] = edge && hidden(j, acc_row(r, h) + e) ? 0.f : x;
+                    }
+                }
+            }
+            tile_add<RT, DP>(acc, planes[1 - second], 32 * j, s[j], lane);
         }
     }
+    float unit = kDown2;
+    if (any_not_finite(acc)) {
+        unit = 1.0f;
+        Redone<DP> r;
+        redo_dkv<DP>(r, a, sp, kv, second, key0, first, tiles, it0, it1, RT, delta, dout, lse, q, k_row, v_row);
+#pragma unroll
+        for (int i = 0; i < NB; ++i) acc[i] = r.x[i];
+    }
     if (!live) return;
-    float *dkr = dk + row * a.k_rs + (size_t)kv * a.k_hs, *dvr = dv + row * a.v_rs + (size_t)kv * a.v_hs;
+    float* dst = second ? dk + row * a.k_rs + (size_t)kv * a.k_hs : dv + row * a.v_rs + (size_t)kv * a.v_hs;
     bool dst_vec = vec;
+    int width = dim;
     if (gridDim.y > 1) {
         const size_t tile = (size_t)blockIdx.y * gridDim.x + (size_t)w.tile0 * a.n_kv + kv;
-        dkr = part + (tile * 2 * kRowsPerWG + key - w.tile * kRowsPerWG) * DP;
-        dvr = dkr + kRowsPerWG * DP;
+        dst = part + ((tile * 2 + 1 - second) * kRowsPerWG + key - w.tile * kRowsPerWG) * DP;
         dst_vec = true;
+        width = DP;
     }
-    const int width = gridDim.y > 1 ? DP : dim;
+    const float by = second ? a.scale : 1.0f;
 #pragma unroll
     for (int i = 0; i < NB; ++i)
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-            const int at = 32 * i + 8 * u + 4 * h;
-            floatx4 x, y;
+            floatx4 x;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                x[e] = ak[i][4 * u + e] * unit * a.scale;
-                y[e] = av[i][4 * u + e] * unit;
-            }
-            store4(dkr, at, width, dst_vec, x);
-            store4(dvr, at, width, dst_vec, y);
+            for (int e = 0; e < 4; ++e) x[e] = acc[i][4 * u + e] * unit * by;
+            store4(dst, 32 * i + 8 * u + 4 * h, width, dst_vec, x);
         }
 }
 
@@ -573,7 +685,7 @@ __global__ __launch_bounds__(256) void attn_split_dkv_join_kernel(PackedAttn a, 
 int attn_split_forward(const PackedAttn& a, uint32_t items, uint32_t budget, float* out, float* lse, const float* q, const float* k,
                        const float* v, float* ws, hipStream_t s) {
     const dim3 grid(items * a.n_kv);
-#define FMLH_LAUNCH(DP) hipLaunchKernelGGL(attn_split_kernel<DP>, grid, dim3(256), 0, s, a, out, lse, q, k, v, ws, budget)
+#define FMLH_LAUNCH(DP) hipLaunchKernelGGL((a.vec ? attn_split_kernel<DP, true> : attn_split_kernel<DP, false>), grid, dim3(256), 0, s, a, out, lse, q, k, v, ws, budget)
     FMLH_BY_DIM(FMLH_LAUNCH);
 #undef FMLH_LAUNCH
     FMLH_LAUNCHED("attn_split_kernel");
@@ -583,7 +695,7 @@ int attn_split_forward(const PackedAttn& a, uint32_t items, uint32_t budget, flo
 int attn_split_dq(const PackedAttn& a, uint32_t tiles, float* dq, float* delta, const float* dout, const float* out, const float* lse,
                   const float* q, const float* k, const float* v, hipStream_t s) {
     const dim3 grid(tiles * a.n_kv);
-#define FMLH_LAUNCH(DP) hipLaunchKernelGGL(attn_split_dq_kernel<DP>, grid, dim3(256), 0, s, a, dq, delta, dout, out, lse, q, k, v)
+#define FMLH_LAUNCH(DP) hipLaunchKernelGGL((a.vec ? attn_split_dq_kernel<DP, true> : attn_split_dq_kernel<DP, false>), grid, dim3(256), 0, s, a, dq, delta, dout, out, lse, q, k, v)
     FMLH_BY_DIM(FMLH_LAUNCH);
 #undef FMLH_LAUNCH
     FMLH_LAUNCHED("attn_split_dq_kernel");
@@ -599,7 +711,7 @@ int attn_split_dkv(const PackedAttn& a, uint32_t tiles, int parts, float* dk, fl
                    const float* lse, const float* q, const float* k, const float* v, float* part, hipStream_t s) {
     const dim3 grid(tiles * a.n_kv, parts);
 #define FMLH_LAUNCH(DP) \
-    hipLaunchKernelGGL(attn_split_dkv_kernel<DP>, grid, dim3(256), 0, s, a, dk, dv, delta, dout, lse, q, k, v, part)
+    hipLaunchKernelGGL((a.vec ? attn_split_dkv_kernel<DP, true> : attn_split_dkv_kernel<DP, false>), grid, dim3(512), 0, s, a, dk, dv, delta, dout, lse, q, k, v, part)
     FMLH_BY_DIM(FMLH_LAUNCH);
 #undef FMLH_LAUNCH
     FMLH_LAUNCHED("attn_split_dkv_kernel");
