@@ -624,6 +624,15 @@ PackedAttn make_args(const fmlh_packed_attention* s) {
 uint32_t row_tiles(const PackedAttn& a, uint32_t per) { return (uint32_t)(((uint64_t)a.q_rows * a.group) / per) + a.n_seq; }
 uint32_t key_tiles(const PackedAttn& a) { return a.k_rows / kRowsPerWG + a.n_seq; }
 
+// Sequences of fewer keys are not cut: joining the ranges costs a launch of 5 us.
+constexpr uint64_t kCutKeys = 512;
+
+// Keys that a sequence has room for, on average (a cache in slabs holds a head's rows one behind the other).
+uint64_t keys_per_sequence(const PackedAttn& a) {
+    const uint64_t n = a.k_rows / a.n_seq;
+    return a.k_hs > a.k_rs ? n / a.n_kv : n;
+}
+
 // How the forward pass cuts its work, by the sizes alone (lengths are the device's to know).
 struct ForwardPlan {
     int per;          // rows per tile: kRowsPerWG, or at most 8 for attn_packed_few_kernel
@@ -639,7 +648,7 @@ ForwardPlan plan_forward(const PackedAttn& a) {
     p.tiles = row_tiles(a, p.per);
     const uint64_t about = std::max<uint64_t>(a.n_seq, (rows + p.per - 1) / p.per) * a.n_kv;
     const uint64_t want = p.per <= 8 ? 1024 : 512;  // work-groups that keep the device busy
-    p.budget = 2 * about <= want && a.k_rows > kRangeKeys ? (uint32_t)(want / a.n_kv) : 0;
+    p.budget = 2 * about <= want && keys_per_sequence(a) >= kCutKeys ? (uint32_t)(want / a.n_kv) : 0;
     return p;
 }
 
@@ -652,7 +661,9 @@ int plan_parts(const PackedAttn& a) {
     const uint64_t want = 1024;          // work-groups that keep the device busy although early keys see more rows than late ones
     const size_t most = size_t(1) << 26;  // floats of partial sums
     const uint64_t fit = std::max<uint64_t>(1, most / std::max<size_t>(1, attn_split_part_floats(a, key_tiles(a))));
-    return (int)std::min<uint64_t>({16, fit, std::max<uint64_t>(1, want / std::max<uint64_t>(1, tiles))});
+    // A part has some tiles of rows to do on average.
+    const uint64_t steps = (uint64_t)a.q_rows / a.n_seq * a.group / 160;
+    return (int)std::min<uint64_t>({16, fit, std::max<uint64_t>(1, steps), std::max<uint64_t>(1, want / std::max<uint64_t>(1, tiles))});
 }
 
 size_t deltas(const PackedAttn& a) { return ((size_t)a.n_kv * a.group * a.q_rows + 3) / 4 * 4; }  // d_i, in whole 16 bytes

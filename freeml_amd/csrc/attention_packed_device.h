@@ -30,9 +30,9 @@ __device__ __forceinline__ Span load_span(const PackedAttn& a, uint32_t s) {
     return p;
 }
 
-// Wave-wide integer sum and maximum (wave_reduce's lane shifts).
+// Wave-wide integer scan (inclusive), sum and maximum, with wave_reduce's lane shifts.
 template <class Op>
-__device__ __forceinline__ int wave_reduce_int(int v, int identity, Op op) {
+__device__ __forceinline__ int wave_scan_int(int v, int identity, Op op) {
 #define FMLH_STEP(CTRL, ROWS) v = op(v, __builtin_amdgcn_update_dpp(identity, v, CTRL, ROWS, 0xf, false))
     FMLH_STEP(0x111, 0xf);
     FMLH_STEP(0x112, 0xf);
@@ -41,13 +41,14 @@ __device__ __forceinline__ int wave_reduce_int(int v, int identity, Op op) {
     FMLH_STEP(0x142, 0xa);
     FMLH_STEP(0x143, 0xc);
 #undef FMLH_STEP
-    return __builtin_amdgcn_readlane(v, 63);
+    return v;
 }
-__device__ __forceinline__ int wave_sum_int(int v) {
-    return wave_reduce_int(v, 0, [](int a, int b) { return a + b; });
+__device__ __forceinline__ int wave_prefix_int(int v) {
+    return wave_scan_int(v, 0, [](int a, int b) { return a + b; });
 }
+__device__ __forceinline__ int wave_sum_int(int v) { return __builtin_amdgcn_readlane(wave_prefix_int(v), 63); }
 __device__ __forceinline__ int wave_max_int(int v) {
-    return wave_reduce_int(v, -0x7fffffff, [](int a, int b) { return max(a, b); });
+    return __builtin_amdgcn_readlane(wave_scan_int(v, -0x7fffffff, [](int a, int b) { return max(a, b); }), 63);
 }
 
 // What a work-group does: tile `tile` of a sequence's `tiles`, and of the `ranges` that the sequence's
@@ -59,6 +60,7 @@ struct Work {
     int range, ranges, per;
 };
 
+constexpr uint32_t kAtOnce = 512;  // work-groups of attention kernels on the device at once
 constexpr int kRangeKeys = 128;  // a range is a multiple of this
 
 // Finds work number `index`, counted in tiles (BY_TILE) or in (tile, range) items.  Sequence s has
@@ -68,7 +70,7 @@ constexpr int kRangeKeys = 128;  // a range is a multiple of this
 // Every wave scans the offsets, 64 sequences at a time.  False behind the last sequence: grids hold
 // sum / per_tile + n_seq tiles and budget items more, never fewer than there are.
 // Up to 64 sequences whose keys are not cut come in the order of their work, most first over all of
-// them: a tile's level falls by one from each to the next, and work number `index` lies on the highest
+// them, where the launch has more work-groups than run at once (below, finding the order only costs 1 us): a tile's level falls by one from each to the next, and work number `index` lies on the highest
 // level T with more than index tiles on it and above.
 template <bool KEYS, bool BY_TILE>
 __device__ __forceinline__ bool find_work(const PackedAttn& a, uint32_t per_tile, uint32_t budget, uint32_t index, Work* w) {
@@ -90,7 +92,7 @@ __device__ __forceinline__ bool find_work(const PackedAttn& a, uint32_t per_tile
         const uint64_t per = (keys / budget + kRangeKeys) / kRangeKeys * kRangeKeys;
         w->per = (int)min(per, (uint64_t)0x40000000);
     }
-    if (!budget && a.n_seq <= 64) {
+    if (!budget && a.n_seq <= 64 && gridDim.x > kAtOnce) {
         if (lane < a.n_seq) p = load_span(a, lane);
         const int n = tiles_of(p);  // at most 2^23, and a level 2^24: sums over 64 lanes stay inside 32 bits
         // Keys that a sequence's last tile sees (rows that see its first tile), in tiles.
@@ -107,19 +109,14 @@ __device__ __forceinline__ bool find_work(const PackedAttn& a, uint32_t per_tile
         const uint64_t level = __ballot(on);
         const uint32_t r = index - above(hi), mine = __builtin_popcountll(level & ((1ull << lane) - 1));
         const int l = __builtin_ctzll(__ballot(on && mine == r));
-        uint32_t upto = n;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const uint32_t x = __shfl_up(upto, d);
-            if (lane >= (uint32_t)d) upto += x;
-        }
-        w->sp.q0 = __shfl(p.q0, l);
-        w->sp.ql = __shfl(p.ql, l);
-        w->sp.k0 = __shfl(p.k0, l);
-        w->sp.kl = __shfl(p.kl, l);
-        w->tiles = __shfl(n, l);
-        w->tile = __shfl(KEYS ? top - lo : n - 1 - (top - lo), l);
-        w->tile0 = w->item0 = __shfl(upto - n, l) + w->tile;
+        const uint32_t upto = wave_prefix_int(n);
+        w->sp.q0 = __builtin_amdgcn_readlane(p.q0, l);
+        w->sp.ql = __builtin_amdgcn_readlane(p.ql, l);
+        w->sp.k0 = __builtin_amdgcn_readlane(p.k0, l);
+        w->sp.kl = __builtin_amdgcn_readlane(p.kl, l);
+        w->tiles = __builtin_amdgcn_readlane(n, l);
+        w->tile = __builtin_amdgcn_readlane(KEYS ? top - lo : n - 1 - (top - lo), l);
+        w->tile0 = w->item0 = __builtin_amdgcn_readlane(upto - n, l) + w->tile;
         w->range = 0;
         w->ranges = 1;
         return true;
@@ -131,25 +128,17 @@ __device__ __forceinline__ bool find_work(const PackedAttn& a, uint32_t per_tile
             if (base + lane < a.n_seq) p = load_span(a, base + lane);
         }
         const uint32_t n = tiles_of(p), r = max(1u, (p.kl + (uint32_t)w->per - 1) / (uint32_t)w->per), items = n * r;
-        uint32_t upto_t = n, upto_i = items;  // inclusive scans
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const uint32_t x = __shfl_up(upto_t, d), y = __shfl_up(upto_i, d);
-            if (lane >= (uint32_t)d) {
-                upto_t += x;
-                upto_i += y;
-            }
-        }
+        const uint32_t upto_t = wave_prefix_int(n), upto_i = wave_prefix_int(items);
         const uint64_t hit = __ballot((BY_TILE ? tiles_before + upto_t : items_before + upto_i) > index);
         if (hit) {
             const int l = __builtin_ctzll(hit);
-            w->sp.q0 = __shfl(p.q0, l);
-            w->sp.ql = __shfl(p.ql, l);
-            w->sp.k0 = __shfl(p.k0, l);
-            w->sp.kl = __shfl(p.kl, l);
-            w->tiles = __shfl(n, l);
-            w->ranges = __shfl(r, l);
-            const uint32_t first_t = tiles_before + __shfl(upto_t - n, l), first_i = items_before + __shfl(upto_i - items, l);
+            w->sp.q0 = __builtin_amdgcn_readlane(p.q0, l);
+            w->sp.ql = __builtin_amdgcn_readlane(p.ql, l);
+            w->sp.k0 = __builtin_amdgcn_readlane(p.k0, l);
+            w->sp.kl = __builtin_amdgcn_readlane(p.kl, l);
+            w->tiles = __builtin_amdgcn_readlane(n, l);
+            w->ranges = __builtin_amdgcn_readlane(r, l);
+            const uint32_t first_t = tiles_before + __builtin_amdgcn_readlane(upto_t - n, l), first_i = items_before + __builtin_amdgcn_readlane(upto_i - items, l);
             w->tile = BY_TILE ? index - first_t : (index - first_i) / w->ranges;
             if (!KEYS) w->tile = w->tiles - 1 - w->tile;  // the last rows see the most keys: they start first
             w->range = BY_TILE ? 0 : (index - first_i) % w->ranges;
@@ -157,8 +146,8 @@ __device__ __forceinline__ bool find_work(const PackedAttn& a, uint32_t per_tile
             w->item0 = first_i + w->tile * w->ranges;
             return true;
         }
-        tiles_before += __shfl(upto_t, 63);
-        items_before += __shfl(upto_i, 63);
+        tiles_before += __builtin_amdgcn_readlane(upto_t, 63);
+        items_before += __builtin_amdgcn_readlane(upto_i, 63);
     }
     return false;
 }
