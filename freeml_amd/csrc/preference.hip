@@ -32,34 +32,94 @@ __device__ __forceinline__ int target_id(const float* target, uint32_t row, uint
     return t > -1.0f && t < (float)vocab ? (int)t : -1;
 }
 
-template <class Op>
-__device__ __forceinline__ float block_reduce(float v, float* sh, float identity, Op op) {
-    v = wave_reduce(v, identity, op);
-    __syncthreads();
-    if (threadIdx.x % kWave == 0) sh[threadIdx.x / kWave] = v;
-    __syncthreads();
-    float r = sh[0];
-    for (unsigned i = 1; i < blockDim.x / kWave; ++i) r = op(r, sh[i]);
-    return r;
+// e^x for x <= 0 (below 2^-126: zero): x log2(e) rounds x twice, 2.3 |x| 2^-24 of the value where expf gives
+// two units for twice the instructions (row_stat_kernel at 1900 rows of 50304: 115 us with expf, @STAT@).
+__device__ __forceinline__ float exp_neg(float x) { return __builtin_amdgcn_exp2f(x * 1.4426950408889634f); }
+
+// The running maximum and sum of exponentials of some values, joined over lanes and waves.
+struct Running {
+    float top = -INFINITY, sum = 0.f;
+    __device__ __forceinline__ void add(const float (&x)[4]) {
+        const float t = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), top);
+        if (t != top) {  // a maximum moves a few times per thread
+            sum *= top == -INFINITY ? 0.f : exp_neg(top - t);
+            top = t;
+        }
+        const float base = top == -INFINITY ? 0.f : top;
+        sum += (exp_neg(x[0] - base) + exp_neg(x[1] - base)) + (exp_neg(x[2] - base) + exp_neg(x[3] - base));
+    }
+    __device__ __forceinline__ void join_wave() {
+        const float t = wave_max(top);
+        sum = wave_sum(top == -INFINITY && !(sum != sum) ? 0.f : sum * expf(top - t));
+        top = t;
+    }
+};
+
+// Four floats at any 4-byte alignment (one load or store of 16 bytes).
+typedef float floatx4 __attribute__((ext_vector_type(4), aligned(4)));
+
+// Calls f(c, count, x) for the row's columns in fours (count 4 at c, the last ones alone, padded with
+// -infinity), spread over `n` threads.  Which thread adds which columns does not go by the row's
+// alignment: equal rows give equal bits wherever they lie.
+template <int UNROLL, class F>
+__device__ __forceinline__ void for_row(const float* z, uint32_t vocab, uint32_t tid, uint32_t n, F f) {
+    const uint32_t body = vocab / 4, rest = vocab % 4;
+    const floatx4* zb = reinterpret_cast<const floatx4*>(z);
+    uint32_t i = tid;
+    for (; i + (UNROLL - 1) * n < body; i += UNROLL * n) {
+        floatx4 v[UNROLL];
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) v[u] = zb[i + u * n];
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) {
+            const float x[4] = {v[u][0], v[u][1], v[u][2], v[u][3]};
+            f(4 * (i + u * n), 4, x);
+        }
+    }
+    for (; i < body; i += n) {
+        const floatx4 v = zb[i];
+        const float x[4] = {v[0], v[1], v[2], v[3]};
+        f(4 * i, 4, x);
+    }
+    if (tid < rest) {
+        const float x[4] = {z[4 * body + tid], -INFINITY, -INFINITY, -INFINITY};
+        f(4 * body + tid, 1, x);
+    }
 }
 
-__global__ void row_stat_kernel(RowStat* __restrict__ stats, const float* __restrict__ target, const float* __restrict__ logits,
-                                uint32_t vocab) {
-    __shared__ float sh[kThreads / kWave];
-    const uint32_t row = blockIdx.x;
+// ROWS rows per work-group, a wave each (short rows), or one row for all its waves.
+template <int ROWS>
+__global__ __launch_bounds__(kThreads) void row_stat_kernel(RowStat* __restrict__ stats, const float* __restrict__ target,
+                                                            const float* __restrict__ logits, uint32_t vocab, uint32_t rows) {
+    __shared__ float sh[kThreads / kWave][2];
+    const uint32_t wave = threadIdx.x / kWave;
+    const uint32_t row = ROWS == 1 ? blockIdx.x : blockIdx.x * ROWS + wave;
+    if (row >= rows) return;
     const int id = target_id(target, row, vocab);
     if (id < 0) {
-        if (threadIdx.x == 0) stats[row] = RowStat{0.0, 0.f, 0.f};
+        if (threadIdx.x % (ROWS == 1 ? kThreads : kWave) == 0) stats[row] = RowStat{0.0, 0.f, 0.f};
         return;
     }
     const float* z = logits + (size_t)row * vocab;
-    float top = -INFINITY;
-    for (uint32_t c = threadIdx.x; c < vocab; c += kThreads) top = fmaxf(top, z[c]);
-    top = block_reduce(top, sh, -INFINITY, [](float a, float b) { return fmaxf(a, b); });
-    float sum = 0.f;
-    for (uint32_t c = threadIdx.x; c < vocab; c += kThreads) sum += expf(z[c] - top);
-    sum = block_reduce(sum, sh, 0.f, [](float a, float b) { return a + b; });
-    if (threadIdx.x == 0) stats[row] = RowStat{(double)(z[id] - top) - log((double)sum), top, 1.0f / sum};
+    const float zt = z[id];
+    Running r;
+    if (ROWS == 1) for_row<4>(z, vocab, threadIdx.x, kThreads, [&](uint32_t, int, const float(&x)[4]) { r.add(x); });
+    else for_row<2>(z, vocab, threadIdx.x % kWave, kWave, [&](uint32_t, int, const float(&x)[4]) { r.add(x); });
+    r.join_wave();
+    float top = r.top, sum = r.sum;
+    if (ROWS == 1) {
+        if (threadIdx.x % kWave == 0) {
+            sh[wave][0] = top;
+            sh[wave][1] = sum;
+        }
+        __syncthreads();
+        top = -INFINITY;
+        for (int i = 0; i < (int)(kThreads / kWave); ++i) top = fmaxf(top, sh[i][0]);
+        sum = 0.f;
+        for (int i = 0; i < (int)(kThreads / kWave); ++i)
+            sum += sh[i][0] == -INFINITY && sh[i][1] == 0.f ? 0.f : sh[i][1] * expf(sh[i][0] - top);
+    }
+    if (threadIdx.x % (ROWS == 1 ? kThreads : kWave) == 0) stats[row] = RowStat{(double)(zt - top) - log((double)sum), top, 1.0f / sum};
 }
 
 // The sum of a sequence's rows, by one wave: lanes take rows in turn, then a fixed tree.
@@ -100,40 +160,72 @@ __global__ void pair_kernel(float* __restrict__ factor, double* __restrict__ pai
 }
 
 // The mean of the pairs' losses: one wave, a fixed order.
-__global__ void pair_mean_kernel(float* __restrict__ loss, const double* __restrict__ pair_loss, uint32_t pairs) {
+__device__ __forceinline__ void pair_mean(float* loss, const double* pair_loss, uint32_t pairs) {
     double t = 0.0;
-    for (uint32_t p = threadIdx.x; p < pairs; p += kWave) t += pair_loss[p];
+    for (uint32_t p = threadIdx.x % kWave; p < pairs; p += kWave) t += pair_loss[p];
 #pragma unroll
     for (int d = 32; d >= 1; d >>= 1) t += __shfl_xor(t, d);
     if (threadIdx.x == 0) loss[0] = (float)(t / pairs);
 }
 
-// The sequence that holds a row: the last offset at or below it (offsets do not fall).  -1: none.
+__global__ void pair_mean_kernel(float* __restrict__ loss, const double* __restrict__ pair_loss, uint32_t pairs) {
+    pair_mean(loss, pair_loss, pairs);
+}
+
+// The sequence that holds a row: the last offset at or below it (offsets do not fall), by 64 lanes.  -1: none.
 __device__ __forceinline__ int row_sequence(const int32_t* off, uint32_t n_seq, uint32_t row) {
     if ((int64_t)row < off[0] || (int64_t)row >= off[n_seq]) return -1;
-    uint32_t lo = 0, hi = n_seq;  // off[lo] <= row < off[hi]
-    while (hi - lo > 1) {
-        const uint32_t mid = (lo + hi) / 2;
-        if ((int64_t)off[mid] <= row) lo = mid;
-        else hi = mid;
+    uint32_t lo = 0, n = n_seq;  // among off[lo] .. off[lo + n - 1], off[lo] <= row
+    while (n > 1) {
+        const uint32_t step = (n + kWave - 1) / kWave, i = min((threadIdx.x % kWave) * step, n - 1);
+        const uint64_t below = __ballot((int64_t)off[lo + i] <= row);
+        const uint32_t last = below ? 63 - __builtin_clzll(below) : 0;  // the last lane at or below
+        const uint32_t at = min(last * step, n - 1);
+        n = min(step, n - at);
+        lo += at;
+        if (step == 1) break;
     }
     return (int)lo;
 }
 
-// grad may be logits: an element is read by the thread that writes it.
-__global__ void pair_gradient_kernel(float* grad, const float* __restrict__ factor, const RowStat* __restrict__ stats,
-                                     const float* __restrict__ target, const float* logits,
-                                     const int32_t* __restrict__ off, uint32_t vocab, uint32_t n_seq) {
-    const uint32_t row = blockIdx.x;
+// grad may be logits: an element is read by the thread that writes it.  The last work-group but the
+// rows' forms the loss.  Rows come in the reverse order of the first pass: what it read last may
+// still lie in the memory-side cache.
+template <int ROWS>
+__global__ __launch_bounds__(kThreads) void pair_gradient_kernel(float* grad, const float* __restrict__ factor, const RowStat* __restrict__ stats,
+                                                                 const float* __restrict__ target, const float* logits,
+                                                                 const int32_t* __restrict__ off, uint32_t vocab, uint32_t rows,
+                                                                 uint32_t n_seq, float* __restrict__ loss,
+                                                                 const double* __restrict__ pair_loss) {
+    if (blockIdx.x == gridDim.x - 1) {
+        if (loss && threadIdx.x < kWave) pair_mean(loss, pair_loss, n_seq / 2);
+        return;
+    }
+    const uint32_t at = ROWS == 1 ? blockIdx.x : blockIdx.x * ROWS + threadIdx.x / kWave;
+    if (at >= rows) return;
+    const uint32_t row = rows - 1 - at;
+    const int id = target_id(target, row, vocab);
+    const RowStat st = stats[row];
     const int s = row_sequence(off, n_seq, row);
     if (s < 0) return;
-    const int id = target_id(target, row, vocab);
     float* g = grad + (size_t)row * vocab;
-    const float f = s & 1 ? -factor[s / 2] : factor[s / 2];
-    const RowStat st = stats[row];
     const float* z = logits + (size_t)row * vocab;
-    for (uint32_t c = threadIdx.x; c < vocab; c += kThreads)
-        g[c] = id < 0 ? 0.f : f * (((int)c == id ? 1.0f : 0.0f) - expf(z[c] - st.top) * st.inv);
+    const uint32_t tid = ROWS == 1 ? threadIdx.x : threadIdx.x % kWave, n = ROWS == 1 ? kThreads : kWave;
+    if (id < 0) {  // nothing to read
+        for (uint32_t i = tid; i < vocab / 4; i += n) reinterpret_cast<floatx4*>(g)[i] = floatx4{0.f, 0.f, 0.f, 0.f};
+        if (tid < vocab % 4) g[vocab / 4 * 4 + tid] = 0.f;
+        return;
+    }
+    const float f = s & 1 ? -factor[s / 2] : factor[s / 2];
+    auto value = [&](uint32_t c, int count, const float(&x)[4]) {
+        floatx4 y;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = f * (((int)(c + e) == id ? 1.0f : 0.0f) - exp_neg(x[e] - st.top) * st.inv);
+        if (count == 4) *reinterpret_cast<floatx4*>(g + c) = y;
+        else g[c] = y[0];
+    };
+    if (ROWS == 1) for_row<4>(z, vocab, tid, n, value);
+    else for_row<2>(z, vocab, tid, n, value);
 }
 
 // Workspace: a RowStat per row, then a double and a float per pair.
@@ -148,9 +240,15 @@ int check(const char* fn, const void* ws, const float* target, const float* logi
     return FMLH_OK;
 }
 
+// Rows of up to 1024 logits: a wave each.
+bool short_rows(uint32_t vocab) { return vocab <= 1024; }
+
 int launch_row_stats(RowStat* stats, const float* target, const float* logits, uint32_t vocab, uint32_t rows) {
     if (rows == 0) return FMLH_OK;
-    hipLaunchKernelGGL(row_stat_kernel, dim3(rows), dim3(kThreads), 0, stream(), stats, target, logits, vocab);
+    if (short_rows(vocab))
+        hipLaunchKernelGGL(row_stat_kernel<4>, dim3((rows + 3) / 4), dim3(kThreads), 0, stream(), stats, target, logits, vocab, rows);
+    else
+        hipLaunchKernelGGL(row_stat_kernel<1>, dim3(rows), dim3(kThreads), 0, stream(), stats, target, logits, vocab, rows);
     FMLH_LAUNCHED("row_stat_kernel");
     return FMLH_OK;
 }
@@ -201,14 +299,17 @@ int fmlh_preference_logits(float* grad, float* loss, float* logp, float* ws, con
     hipLaunchKernelGGL(pair_kernel, dim3((pairs + 3) / 4), dim3(kThreads), 0, stream(), factor, pair_loss, logp, stats, off,
                        ref_logp, rows, pairs, beta, smoothing);
     FMLH_LAUNCHED("pair_kernel");
-    if (loss) {
+    if (grad && rows) {
+#define FMLH_GRADIENT(ROWS)                                                                                                     \
+    hipLaunchKernelGGL(pair_gradient_kernel<ROWS>, dim3((rows + ROWS - 1) / ROWS + 1), dim3(kThreads), 0, stream(), grad, factor, \
+                       stats, target, logits, off, vocab, rows, 2 * pairs, loss, pair_loss)
+        if (short_rows(vocab)) FMLH_GRADIENT(4);
+        else FMLH_GRADIENT(1);
+#undef FMLH_GRADIENT
+        FMLH_LAUNCHED("pair_gradient_kernel");
+    } else if (loss) {
         hipLaunchKernelGGL(pair_mean_kernel, dim3(1), dim3(kWave), 0, stream(), loss, pair_loss, pairs);
         FMLH_LAUNCHED("pair_mean_kernel");
-    }
-    if (grad && rows) {
-        hipLaunchKernelGGL(pair_gradient_kernel, dim3(rows), dim3(kThreads), 0, stream(), grad, factor, stats, target, logits, off,
-                           vocab, 2 * pairs);
-        FMLH_LAUNCHED("pair_gradient_kernel");
     }
     return FMLH_OK;
 }

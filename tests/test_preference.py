@@ -1,11 +1,12 @@
 """The preference loss on packed pairs and the sequences' log-probabilities against the formula in
 64 bits.
 
-Tolerances (u = 2^-24): a row's sum of n exponentials is off by at most (n + 4) u relative (exp is
-within two units of its value, its argument z - max rounded once: |z - max| u more), so its log-probability by
-(n + 4 + R) u + 2 u R with R the largest |z - max|; a sequence's log-probability by the sum of its rows' and one rounding.
+Tolerances (u = 2^-24): a row's sum of n exponentials is off by at most (n + 4) u relative (the base-2
+exponential is within two units of its value) and 3 |z - max| u more (z - max is rounded, multiplied by a
+rounded log2(e), and rounded again), so its log-probability by (n + 4 + 3 R) u and 2 u R with R the largest |z - max|; a sequence's log-probability by the sum of its rows' and one rounding.
 x is off by beta times its two sequences' bounds, a factor by beta / pairs times a quarter of that (the
-sigmoid's slope) and a rounding, a gradient element by the factor's and the softmax's error.
+sigmoid's slope) and a rounding, a gradient element by the factor's and the softmax's error
+(its own exponential's 3 R u and its sum's 3 R u).
 """
 import numpy as np
 import pytest
@@ -38,7 +39,7 @@ def reference(off, z, t, ref, beta, smoothing):
     ok = ids >= 0
     row = np.where(ok, (z64 - top)[np.arange(len(t)), np.maximum(ids, 0)] - np.log(e.sum(1)), 0.0)
     R = np.where(np.isfinite(z64), top - z64, 0.0).max(1)
-    b_row = np.where(ok, (V + 4 + 3 * R) * U, 0.0)
+    b_row = np.where(ok, (V + 4 + 5 * R) * U, 0.0)
     lp = np.array([row[a:b].sum() for a, b in zip(off, off[1:])])
     b_lp = np.array([b_row[a:b].sum() for a, b in zip(off, off[1:])])
     out = dict(lp=lp, b_lp=b_lp + np.abs(lp) * U)
@@ -57,7 +58,7 @@ def reference(off, z, t, ref, beta, smoothing):
         sign = f[s // 2] * (1 if s % 2 == 0 else -1)
         grad[a:b] = sign * (onehot - soft)[a:b] * ok[a:b, None]
         b_grad[a:b] = ((beta / P * b_x[s // 2] / 4 + 4 * U * abs(sign)) * np.abs((onehot - soft)[a:b]) +
-                       abs(sign) * (soft * ((V + 8 + R)[:, None] * U) + 2 * U * onehot)[a:b]) * ok[a:b, None]
+                       abs(sign) * (soft * ((V + 8 + 6 * R)[:, None] * U) + 2 * U * onehot)[a:b]) * ok[a:b, None]
     out.update(loss=loss.mean(), b_loss=b_x.mean() + np.abs(loss).mean() * 4 * U, grad=grad, b_grad=b_grad, x=x)
     return out
 
@@ -105,12 +106,15 @@ def test_loss_and_gradient(lens, vocab, smoothing):
 @pytest.mark.parametrize("vocab", [65, 1001, 4100, 50304])
 @pytest.mark.parametrize("shift", [0, 1, 2])
 def test_gradient_in_place_and_any_alignment(vocab, shift):
+    """In place, and at any alignment: the same bits."""
     off, rows, z, t, ref = inputs([6, 5, 2, 9], vocab, seed=1, extra=(0, 3))
     a = run(off, rows, z, t, ref)[0]
     b = run(off, rows, z, t, ref, in_place=True, shift=shift)[0]
     n = off[-1]
     np.testing.assert_array_equal(a[:n], b[:n])
     np.testing.assert_array_equal(b[n:], z[n:])
+    r = reference(off, z, t, ref, np.float64(np.float32(0.1)), 0.0)
+    close(a, r["grad"], r["b_grad"], "grad")
 
 
 @pytest.mark.gpu
