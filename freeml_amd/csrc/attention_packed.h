@@ -17,14 +17,13 @@ struct PackedAttn {
 };
 
 // The kernels on the bf16 matrix cores (attention_packed_split.hip).  Grids hold `items` / `tiles` per
-// key head; ws and part are workspace.
+// key head; ws, delta and sums are workspace.
 int attn_split_forward(const PackedAttn& a, uint32_t items, uint32_t budget, float* out, float* lse, const float* q, const float* k,
                        const float* v, float* ws, hipStream_t s);
-int attn_split_dq(const PackedAttn& a, uint32_t tiles, float* dq, float* delta, const float* dout, const float* out, const float* lse,
-                  const float* q, const float* k, const float* v, hipStream_t s);
-// Floats that one of the parts of attn_split_dkv leaves (parts > 1).
-size_t attn_split_part_floats(const PackedAttn& a, uint32_t tiles);
-int attn_split_dkv(const PackedAttn& a, uint32_t tiles, int parts, float* dk, float* dv, const float* delta, const float* dout,
-                   const float* lse, const float* q, const float* k, const float* v, float* part, hipStream_t s);
+// Floats that one of the parts of dk and dv leaves in `sums` (parts > 1).
+size_t attn_split_part_floats(const PackedAttn& a, uint32_t key_tiles);
+int attn_split_backward(const PackedAttn& a, uint32_t row_tiles, uint32_t key_tiles, int parts, float* dq, float* dk, float* dv,
+                        float* delta, const float* dout, const float* out, const float* lse, const float* q, const float* k,
+                        const float* v, float* sums, hipStream_t s);
 
 }  // namespace fmlh

@@ -25,55 +25,6 @@ namespace fmlh {
 
 namespace {
 
-// NaN where a value is infinite or NaN, else 0.
-__device__ __forceinline__ float not_finite(floatx4 v) { return (v[0] + v[1] + v[2] + v[3]) * 0.f; }
-
-// Copies rows [first, first + R) of a matrix (row stride rs) into LDS rows of LD floats, DP of
-// them filled; rows from `rows` on are zero.  Returns NaN where a value is not finite.
-template <int R, int DP, int LD>
-__device__ __forceinline__ float stage_rows(float* lds, const float* base, size_t rs, uint32_t first, uint32_t rows, int dim,
-                                            bool vec) {
-    constexpr int U = DP / 4;
-    float bad = 0.f;
-    for (int e = threadIdx.x; e < R * U; e += 256) {
-        const uint32_t r = first + e / U;
-        const int d = 4 * (e % U);
-        floatx4 v = {0.f, 0.f, 0.f, 0.f};
-        if (r < rows) v = load4(base + (size_t)r * rs, d, dim, vec);
-        bad += not_finite(v);
-        *reinterpret_cast<floatx4*>(lds + (e / U) * LD + d) = v;
-    }
-    return bad;
-}
-
-// S (32 x 32) = A B^T over DP dims: A's rows from LDS (row stride LD), B's row of lane column c in
-// registers (dims h DP / 2 ..).  The matrix core's two k of a step are dims u and DP / 2 + u.
-template <int DP, int LD>
-__device__ __forceinline__ floatx16 lds_rows_product(const float* lds_rows, const float (&b)[DP / 2], int h, int c) {
-    floatx16 s;
-#pragma unroll
-    for (int r = 0; r < 16; ++r) s[r] = 0.f;
-    const float* row = lds_rows + c * LD + h * (DP / 2);
-#pragma unroll
-    for (int u = 0; u < DP / 2; u += 4) {
-        const floatx4 x = *reinterpret_cast<const floatx4*>(row + u);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s = __builtin_amdgcn_mfma_f32_32x32x2f32(x[e], b[u + e], s, 0, 0, 0);
-    }
-    return s;
-}
-
-// acc (dims x 32 columns) += X^T w, X 32 rows in LDS, w their 32 x 32 weights in accumulator layout.
-template <int DP, int LD>
-__device__ __forceinline__ void add_product(floatx16 (&acc)[DP / 32], const float* lds_rows, const floatx16& w, int h, int c) {
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-        const float* x = lds_rows + acc_row(r, h) * LD + c;
-#pragma unroll
-        for (int i = 0; i < DP / 32; ++i) acc[i] = __builtin_amdgcn_mfma_f32_32x32x2f32(x[32 * i], w[r], acc[i], 0, 0, 0);
-    }
-}
-
 // ---- few rows over many keys -------------------------------------------------------------------
 
 // Single tokens over a cache: with RT rows (the heads of a group, a few queries) the keys' and values'
@@ -223,7 +174,7 @@ __global__ __launch_bounds__(256) void attn_packed_few_kernel(PackedAttn a, floa
             store4(out + row * a.o_rs + head * dim, d, dim, a.vec, x * inv);
             if (lse && d == 0) lse[at] = (top + log2f(sum)) * kLn2;
         } else {
-            store4(part.o + t * dim, d, dim, false, x);
+            store4(part.o + t * padded_dim(dim), d, dim, true, x);
             if (d == 0) {
                 part.ml[2 * t] = top;
                 part.ml[2 * t + 1] = sum;
@@ -264,7 +215,7 @@ __global__ __launch_bounds__(256) void attn_packed_join_kernel(PackedAttn a, flo
             for (int i = 0; i < 8; ++i)
 #pragma unroll
                 for (int e = 0; e < 2; ++e)
-                    y[i][e] = lane + 64 * e < dim ? part.o[((size_t)min(z0 + i0 + i, tl.ranges - 1) * TILE + t) * dim + lane + 64 * e] : 0.f;
+                    y[i][e] = lane + 64 * e < dim ? part.o[((size_t)min(z0 + i0 + i, tl.ranges - 1) * TILE + t) * padded_dim(dim) + lane + 64 * e] : 0.f;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const float c = __shfl(corr, i0 + i);
@@ -283,292 +234,6 @@ __global__ __launch_bounds__(256) void attn_packed_join_kernel(PackedAttn a, flo
     if (lse && lane == 0) lse[head * a.q_rows + row] = (top + log2f(sum)) * kLn2;
 }
 
-// ---- forward ---------------------------------------------------------------------------------
-
-// A work-group per 128 rows of one (sequence, key head), 32 per wave, a row per lane column c; the
-// products are taken transposed, S^T = K Q^T and O^T += V^T P^T, so that a lane's probabilities
-// are the matrix core's operand as they stand.
-template <int DP>
-__global__ __launch_bounds__(256) void attn_packed_kernel(PackedAttn a, float* __restrict__ out, float* __restrict__ lse,
-                                                          const float* __restrict__ q, const float* __restrict__ k,
-                                                          const float* __restrict__ v, float* __restrict__ ws, uint32_t budget) {
-    constexpr int KT = 32, KL = DP + 4, VL = DP + 8;
-    __shared__ __attribute__((aligned(16))) float ks[KT * KL];
-    __shared__ __attribute__((aligned(16))) float vs[KT * VL];
-    __shared__ int bad_tile;  // the last tile whose values are not all finite, + 1
-    const int kv = blockIdx.x % a.n_kv;
-    Work w;
-    if (!find_work<false, false>(a, kRowsPerWG, budget, blockIdx.x / a.n_kv, &w)) return;
-    const RowTile tl = row_tile(a, w, kRowsPerWG);
-    if (w.range >= tl.ranges) return;
-    const Span sp = w.sp;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, c = lane & 31;
-    const int dim = a.head_dim, group = a.group, rows = tl.rows, shift = tl.shift, k_begin = tl.k_begin, k_end = tl.k_end;
-    const int rho = tl.rho0 + wave * kRowsPerWave + c;
-    const bool live = rho < rows;
-    const int qi = (live ? rho : rows - 1) / group, head = kv * group + (live ? rho : rows - 1) % group;
-    const int limit = qi + shift;  // last key this row sees
-    const float* kb = k + (size_t)sp.k0 * a.k_rs + (size_t)kv * a.k_hs;
-    const float* vb = v + (size_t)sp.k0 * a.v_rs + (size_t)kv * a.v_hs;
-
-    float qr[DP / 2];
-    const float* q_row = q + (size_t)(sp.q0 + qi) * a.q_rs + (size_t)head * dim;
-#pragma unroll
-    for (int u = 0; u < DP / 2; u += 4) {
-        const floatx4 x = load4(q_row, h * (DP / 2) + u, dim, a.vec);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) qr[u + e] = x[e];
-    }
-    floatx16 o[DP / 32];
-#pragma unroll
-    for (int i = 0; i < DP / 32; ++i)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) o[i][r] = 0.f;
-    float m = -INFINITY, l = 0.f;
-    const float factor = a.scale * kLog2e;
-    if (threadIdx.x == 0) bad_tile = 0;
-    for (int t0 = k_begin; t0 < k_end; t0 += KT) {
-        __syncthreads();
-        stage_rows<KT, DP, KL>(ks, kb, a.k_rs, t0, k_end, dim, a.vec);
-        if (stage_rows<KT, DP, VL>(vs, vb, a.v_rs, t0, k_end, dim, a.vec) != 0.f) bad_tile = t0 + 1;
-        __syncthreads();
-        floatx16 s = lds_rows_product<DP, KL>(ks, qr, h, c);
-        uint32_t seen = 0;
-        float top = m;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            s[r] *= factor;
-            if (t0 + acc_row(r, h) <= min(limit, k_end - 1)) {
-                seen |= 1u << r;
-                top = fmaxf(top, s[r]);
-            } else {
-                s[r] = -INFINITY;
-            }
-        }
-        top = fmaxf(top, __shfl_xor(top, 32));
-        const float base = top == -INFINITY ? 0.f : top;  // nothing seen, or scores of -inf alone
-        const float corr = exp2f(m - base);
-        m = top;
-        float sum = 0.f;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            s[r] = exp2f(s[r] - base);
-            sum += s[r];
-        }
-        l = l * corr + sum;
-#pragma unroll
-        for (int i = 0; i < DP / 32; ++i)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) o[i][r] *= corr;
-        if (bad_tile == t0 + 1 && __ballot(seen != 0xffffu)) add_seen<DP>(o, s, seen, h, c, DP, true, [&](int n) { return vs + n * VL; });
-        else add_product<DP, VL>(o, vs, s, h, c);
-    }
-    l += __shfl_xor(l, 32);
-    if (!live) return;
-    const size_t at = (size_t)head * a.q_rows + sp.q0 + qi;
-    float inv = limit < 0 || sp.kl == 0 ? 0.f : 1.0f / l;
-    float* dst = out + (size_t)(sp.q0 + qi) * a.o_rs + (size_t)head * dim;
-    int vec = a.vec;
-    if (tl.ranges > 1) {
-        const int t = rho - tl.rho0;
-        const Partials part = partials(ws, a.n_kv, kv, gridDim.x / a.n_kv, w.item0 + w.range, kRowsPerWG, dim);
-        inv = 1.0f;
-        dst = part.o + t * dim;
-        vec = 0;
-        if (h == 0) {
-            part.ml[2 * t] = m;
-            part.ml[2 * t + 1] = l;
-        }
-    } else if (lse && h == 0) {
-        lse[at] = (m + log2f(l)) * kLn2;
-    }
-#pragma unroll
-    for (int i = 0; i < DP / 32; ++i)
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            floatx4 x;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] = o[i][4 * u + e] * inv;
-            store4(dst, 32 * i + 8 * u + 4 * h, dim, vec, x);
-        }
-}
-
-// ---- backward --------------------------------------------------------------------------------
-
-// dq, and d_i of every row for the kernel below: work-groups and lanes as in the forward pass,
-// dQ^T += K^T dS^T.
-template <int DP>
-__global__ __launch_bounds__(256) void attn_packed_dq_kernel(PackedAttn a, float* __restrict__ dq, float* __restrict__ delta,
-                                                             const float* __restrict__ dout, const float* __restrict__ out,
-                                                             const float* __restrict__ lse, const float* __restrict__ q,
-                                                             const float* __restrict__ k, const float* __restrict__ v) {
-    constexpr int KT = 32, LD = DP + 4;
-    __shared__ __attribute__((aligned(16))) float ks[KT * LD];
-    __shared__ __attribute__((aligned(16))) float vs[KT * LD];
-    __shared__ int bad_tile;
-    const int kv = blockIdx.x % a.n_kv;
-    Work w;
-    if (!find_work<false, true>(a, kRowsPerWG, 0, blockIdx.x / a.n_kv, &w)) return;
-    const RowTile tl = row_tile(a, w, kRowsPerWG);
-    const Span sp = w.sp;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, c = lane & 31;
-    const int dim = a.head_dim, group = a.group, rows = tl.rows, shift = tl.shift, nkeys = tl.nkeys;
-    const int rho = tl.rho0 + wave * kRowsPerWave + c;
-    const bool live = rho < rows;
-    const int qi = (live ? rho : rows - 1) / group, head = kv * group + (live ? rho : rows - 1) % group;
-    const int limit = qi + shift;  // last key this row sees
-    const float* kb = k + (size_t)sp.k0 * a.k_rs + (size_t)kv * a.k_hs;
-    const float* vb = v + (size_t)sp.k0 * a.v_rs + (size_t)kv * a.v_hs;
-
-    float qr[DP / 2], gr[DP / 2];
-    const float* q_row = q + (size_t)(sp.q0 + qi) * a.q_rs + (size_t)head * dim;
-    const float* g_row = dout + (size_t)(sp.q0 + qi) * a.o_rs + (size_t)head * dim;
-    const float* o_row = out + (size_t)(sp.q0 + qi) * a.o_rs + (size_t)head * dim;
-    float d = 0.f;
-#pragma unroll
-    for (int u = 0; u < DP / 2; u += 4) {
-        const int at = h * (DP / 2) + u;
-        const floatx4 x = load4(q_row, at, dim, a.vec), g = load4(g_row, at, dim, a.vec), y = load4(o_row, at, dim, a.vec);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            qr[u + e] = x[e];
-            gr[u + e] = g[e];
-            d += g[e] * y[e];
-        }
-    }
-    d += __shfl_xor(d, 32);
-    const size_t stat = (size_t)head * a.q_rows + sp.q0 + qi;
-    if (live && h == 0) delta[stat] = d;
-    const float lse2 = lse[stat] * kLog2e;
-    floatx16 acc[DP / 32];
-#pragma unroll
-    for (int i = 0; i < DP / 32; ++i)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) acc[i][r] = 0.f;
-    const float factor = a.scale * kLog2e;
-    if (threadIdx.x == 0) bad_tile = 0;
-    for (int t0 = 0; t0 < nkeys; t0 += KT) {
-        __syncthreads();
-        if (stage_rows<KT, DP, LD>(ks, kb, a.k_rs, t0, nkeys, dim, a.vec) != 0.f) bad_tile = t0 + 1;
-        stage_rows<KT, DP, LD>(vs, vb, a.v_rs, t0, nkeys, dim, a.vec);
-        __syncthreads();
-        const floatx16 s = lds_rows_product<DP, LD>(ks, qr, h, c);
-        floatx16 ds = lds_rows_product<DP, LD>(vs, gr, h, c);
-        uint32_t seen = 0;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            const bool on = t0 + acc_row(r, h) <= limit;
-            ds[r] = on ? exp2f(s[r] * factor - lse2) * (ds[r] - d) * a.scale : 0.f;
-            seen |= (on ? 1u : 0u) << r;
-        }
-        if (bad_tile == t0 + 1 && __ballot(seen != 0xffffu)) add_seen<DP>(acc, ds, seen, h, c, DP, true, [&](int n) { return ks + n * LD; });
-        else add_product<DP, LD>(acc, ks, ds, h, c);
-    }
-    if (!live) return;
-    float* dst = dq + (size_t)(sp.q0 + qi) * a.q_rs + (size_t)head * dim;
-#pragma unroll
-    for (int i = 0; i < DP / 32; ++i)
-#pragma unroll
-        for (int u = 0; u < 4; ++u)
-            store4(dst, 32 * i + 8 * u + 4 * h, dim, a.vec,
-                   floatx4{acc[i][4 * u], acc[i][4 * u + 1], acc[i][4 * u + 2], acc[i][4 * u + 3]});
-}
-
-// dk and dv: a work-group per 128 keys of one (sequence, key head), 32 per wave, a key per lane
-// column, K and V in registers; the rows of the group's heads stream through LDS, one head after
-// the other: S = Q K^T, dP = dO V^T, dV^T += dO^T P, dK^T += Q^T dS.
-template <int DP>
-__global__ __launch_bounds__(256) void attn_packed_dkv_kernel(PackedAttn a, float* __restrict__ dk, float* __restrict__ dv,
-                                                              const float* __restrict__ delta, const float* __restrict__ dout,
-                                                              const float* __restrict__ lse, const float* __restrict__ q,
-                                                              const float* __restrict__ k, const float* __restrict__ v) {
-    constexpr int RT = 32, LD = DP + 4;
-    __shared__ __attribute__((aligned(16))) float qs[RT * LD];
-    __shared__ __attribute__((aligned(16))) float gs[RT * LD];
-    __shared__ __attribute__((aligned(16))) float stats[2][RT];
-    __shared__ int bad_tile;
-    const int kv = blockIdx.x % a.n_kv;
-    Work w;
-    if (!find_work<true, true>(a, kRowsPerWG, 0, blockIdx.x / a.n_kv, &w)) return;
-    const Span sp = w.sp;
-    const int tile = w.tile;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, c = lane & 31;
-    const int dim = a.head_dim, group = a.group;
-    const int key = tile * kRowsPerWG + wave * kRowsPerWave + c;
-    const bool live = key < (int)sp.kl;
-    const int shift = (int)sp.kl - (int)sp.ql;
-    const size_t row = sp.k0 + (live ? key : (int)sp.kl - 1);
-    float kr[DP / 2], vr[DP / 2];
-#pragma unroll
-    for (int u = 0; u < DP / 2; u += 4) {
-        const int at = h * (DP / 2) + u;
-        const floatx4 x = load4(k + row * a.k_rs + (size_t)kv * a.k_hs, at, dim, a.vec);
-        const floatx4 y = load4(v + row * a.v_rs + (size_t)kv * a.v_hs, at, dim, a.vec);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            kr[u + e] = x[e];
-            vr[u + e] = y[e];
-        }
-    }
-    floatx16 ak[DP / 32], av[DP / 32];
-#pragma unroll
-    for (int i = 0; i < DP / 32; ++i)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) ak[i][r] = av[i][r] = 0.f;
-    const float factor = a.scale * kLog2e;
-    if (threadIdx.x == 0) bad_tile = 0;
-    const int first = max(0, tile * kRowsPerWG - shift) / RT * RT;  // the first row that sees a key of the tile
-    int pass = 0;
-    for (int g = 0; g < group; ++g) {
-        const int head = kv * group + g;
-        const float* qb = q + (size_t)sp.q0 * a.q_rs + (size_t)head * dim;
-        const float* gb = dout + (size_t)sp.q0 * a.o_rs + (size_t)head * dim;
-        const size_t stat = (size_t)head * a.q_rows + sp.q0;
-        for (int i0 = first; i0 < (int)sp.ql; i0 += RT) {
-            ++pass;
-            __syncthreads();
-            float bad = stage_rows<RT, DP, LD>(qs, qb, a.q_rs, i0, sp.ql, dim, a.vec);
-            bad += stage_rows<RT, DP, LD>(gs, gb, a.o_rs, i0, sp.ql, dim, a.vec);
-            if (threadIdx.x < RT) {
-                const bool in = i0 + threadIdx.x < sp.ql;
-                stats[0][threadIdx.x] = in ? lse[stat + i0 + threadIdx.x] * kLog2e : 0.f;
-                stats[1][threadIdx.x] = in ? delta[stat + i0 + threadIdx.x] : 0.f;
-            }
-            if (bad != 0.f) bad_tile = pass;
-            __syncthreads();
-            floatx16 p = lds_rows_product<DP, LD>(qs, kr, h, c);
-            floatx16 ds = lds_rows_product<DP, LD>(gs, vr, h, c);
-            uint32_t seen = 0;
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int i = acc_row(r, h);
-                const bool on = key <= i0 + i + shift && i0 + i < (int)sp.ql;
-                p[r] = on ? exp2f(p[r] * factor - stats[0][i]) : 0.f;
-                ds[r] = on ? p[r] * (ds[r] - stats[1][i]) * a.scale : 0.f;
-                seen |= (on ? 1u : 0u) << r;
-            }
-            if (bad_tile == pass && __ballot(seen != 0xffffu)) {
-                add_seen<DP>(av, p, seen, h, c, DP, true, [&](int n) { return gs + n * LD; });
-                add_seen<DP>(ak, ds, seen, h, c, DP, true, [&](int n) { return qs + n * LD; });
-            } else {
-                add_product<DP, LD>(av, gs, p, h, c);
-                add_product<DP, LD>(ak, qs, ds, h, c);
-            }
-        }
-    }
-    if (!live) return;
-    float* dkr = dk + row * a.k_rs + (size_t)kv * a.k_hs;
-    float* dvr = dv + row * a.v_rs + (size_t)kv * a.v_hs;
-#pragma unroll
-    for (int i = 0; i < DP / 32; ++i)
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            const int at = 32 * i + 8 * u + 4 * h;
-            store4(dkr, at, dim, a.vec, floatx4{ak[i][4 * u], ak[i][4 * u + 1], ak[i][4 * u + 2], ak[i][4 * u + 3]});
-            store4(dvr, at, dim, a.vec, floatx4{av[i][4 * u], av[i][4 * u + 1], av[i][4 * u + 2], av[i][4 * u + 3]});
-        }
-}
-
 // ---- host ------------------------------------------------------------------------------------
 
 // A launch's threads stay inside 32 bits.
@@ -582,7 +247,10 @@ int check_shape(const char* fn, const fmlh_packed_attention* s) {
     FMLH_REQUIRE(s->q_rows <= kMaxRows && s->k_rows <= kMaxRows, "%s: more than 2^30 rows", fn);
     FMLH_REQUIRE(s->n_seq <= kMaxSeqs, "%s: more than 2^22 sequences", fn);
     FMLH_REQUIRE((uint64_t)s->q_rows * (s->n_head / s->n_kv_head) <= kMaxRows, "%s: more than 2^30 rows of a group", fn);
-    FMLH_REQUIRE(s->scale == s->scale && s->scale - s->scale == 0.f, "%s: scale is not finite", fn);
+    // The split kernels carry scale 2^-48 in one factor.
+    const float size = s->scale < 0 ? -s->scale : s->scale;
+    FMLH_REQUIRE(size == 0.f || (size >= 0x1p-60f && size <= 0x1p60f), "%s: scale %g is neither 0 nor of 2^-60 .. 2^60", fn,
+                 (double)s->scale);
     const size_t row = (size_t)s->n_head * s->head_dim;
     FMLH_REQUIRE(s->q_rs >= row && s->o_rs >= row, "%s: rows of q (%zu) and out (%zu) hold %zu floats", fn, s->q_rs, s->o_rs,
                  row);
@@ -647,8 +315,8 @@ ForwardPlan plan_forward(const PackedAttn& a) {
     p.per = per_seq > 8 ? kRowsPerWG : per_seq > 4 ? 8 : per_seq > 2 ? 4 : per_seq > 1 ? 2 : 1;
     p.tiles = row_tiles(a, p.per);
     const uint64_t about = std::max<uint64_t>(a.n_seq, (rows + p.per - 1) / p.per) * a.n_kv;
-    const uint64_t want = p.per <= 8 ? 1024 : 512;  // work-groups that keep the device busy
-    p.budget = 2 * about <= want && keys_per_sequence(a) >= kCutKeys ? (uint32_t)(want / a.n_kv) : 0;
+    const uint64_t want = p.per <= 8 ? 1024 : (getenv("W") ? atoi(getenv("W")) : 512);  // work-groups that keep the device busy
+    p.budget = (getenv("R") ? atoi(getenv("R")) : 2) * about <= 2 * want && keys_per_sequence(a) >= kCutKeys ? (uint32_t)(want / a.n_kv) : 0;
     return p;
 }
 
@@ -671,7 +339,7 @@ size_t deltas(const PackedAttn& a) { return ((size_t)a.n_kv * a.group * a.q_rows
 size_t workspace(const PackedAttn& a, bool backward) {
     if (a.n_seq == 0) return 0;
     const ForwardPlan p = plan_forward(a);
-    const size_t forward = p.budget ? (size_t)a.n_kv * (p.tiles + p.budget) * p.per * (a.head_dim + 2) : 0;
+    const size_t forward = p.budget ? (size_t)a.n_kv * (p.tiles + p.budget) * p.per * (padded_dim(a.head_dim) + 2) : 0;
     if (!backward) return forward;
     const int parts = plan_parts(a);
     return std::max(forward, deltas(a) + (parts > 1 ? parts * attn_split_part_floats(a, key_tiles(a)) : 0));
@@ -682,14 +350,6 @@ size_t workspace(const PackedAttn& a, bool backward) {
 }  // namespace fmlh
 
 using namespace fmlh;
-
-#define FMLH_BY_DIM(LAUNCH)                        \
-    do {                                           \
-        if (a.head_dim <= 32) LAUNCH(32);          \
-        else if (a.head_dim <= 64) LAUNCH(64);     \
-        else if (a.head_dim <= 96) LAUNCH(96);     \
-        else LAUNCH(128);                          \
-    } while (0)
 
 extern "C" {
 
@@ -712,6 +372,7 @@ int fmlh_attention_packed(const fmlh_packed_attention* shape, float* out, float*
     const size_t need = workspace(a, false);
     FMLH_REQUIRE(need == 0 || (ws && ws_floats >= need), "%s: a workspace of %zu floats is needed", fn, need);
     a.vec = a.vec && aligned16(q) && aligned16(k) && aligned16(v) && aligned16(out);
+    FMLH_REQUIRE(need == 0 || (uintptr_t)ws % 16 == 0, "%s: the workspace is not 16-byte aligned", fn);
     const ForwardPlan plan = plan_forward(a);
     const uint32_t items = plan.tiles + plan.budget;
     FMLH_REQUIRE((uint64_t)items * a.n_kv <= kMaxGroups, "%s: more than 2^23 tiles of rows", fn);
@@ -733,15 +394,8 @@ int fmlh_attention_packed(const fmlh_packed_attention* shape, float* out, float*
 #undef FMLH_FEW_ROWS
 #undef FMLH_FEW
         FMLH_LAUNCHED("attn_packed_few_kernel");
-    } else if (!getenv("FMLH_PLAIN")) {
-        FMLH_TRY(attn_split_forward(a, items, plan.budget, out, lse, q, k, v, ws, stream()));
     } else {
-#define FMLH_LAUNCH(DP)                                                                                                \
-    hipLaunchKernelGGL(attn_packed_kernel<DP>, dim3(items * a.n_kv), dim3(256), 0, stream(), a, out, lse, q, k, v, ws, \
-                       plan.budget)
-        FMLH_BY_DIM(FMLH_LAUNCH);
-#undef FMLH_LAUNCH
-        FMLH_LAUNCHED("attn_packed_kernel");
+        FMLH_TRY(attn_split_forward(a, items, plan.budget, out, lse, q, k, v, ws, stream()));
     }
     if (plan.budget) {
 #define FMLH_JOIN(TILE)                                                                                                      \
@@ -773,32 +427,14 @@ int fmlh_attention_packed_backward(const fmlh_packed_attention* shape, float* dq
     const int parts = plan_parts(a);
     const size_t need = deltas(a) + (parts > 1 ? parts * attn_split_part_floats(a, key_tiles(a)) : 0);
     FMLH_REQUIRE(need == 0 || (ws && ws_floats >= need), "%s: a workspace of %zu floats is needed", fn, need);
-    FMLH_REQUIRE((uint64_t)std::max(row_tiles(a, kRowsPerWG), key_tiles(a)) * a.n_kv <= kMaxGroups, "%s: more than 2^23 tiles of rows or keys", fn);
+    FMLH_REQUIRE(((uint64_t)row_tiles(a, kRowsPerWG) + (uint64_t)key_tiles(a) * parts) * a.n_kv <= kMaxGroups / 2 &&
+                     (uint64_t)a.q_rows * shape->n_head <= (uint64_t(1) << 27),
+                 "%s: more than 2^22 tiles of rows and keys, or 2^27 rows of heads", fn);
     a.vec = a.vec && aligned16(q) && aligned16(k) && aligned16(v) && aligned16(out) && aligned16(dout) && aligned16(dq) &&
             aligned16(dk) && aligned16(dv);
     FMLH_REQUIRE((uintptr_t)ws % 16 == 0, "%s: the workspace is not 16-byte aligned", fn);
-    if (!getenv("FMLH_PLAIN")) {
-        if (shape->q_rows) FMLH_TRY(attn_split_dq(a, row_tiles(a, kRowsPerWG), dq, ws, dout, out, lse, q, k, v, stream()));
-        if (shape->k_rows) FMLH_TRY(attn_split_dkv(a, key_tiles(a), parts, dk, dv, ws, dout, lse, q, k, v, ws + deltas(a), stream()));
-        return FMLH_OK;
-    }
-    if (shape->q_rows) {
-        const dim3 grid(row_tiles(a, kRowsPerWG) * a.n_kv);
-#define FMLH_LAUNCH(DP) \
-    hipLaunchKernelGGL(attn_packed_dq_kernel<DP>, grid, dim3(256), 0, stream(), a, dq, ws, dout, out, lse, q, k, v)
-        FMLH_BY_DIM(FMLH_LAUNCH);
-#undef FMLH_LAUNCH
-        FMLH_LAUNCHED("attn_packed_dq_kernel");
-    }
-    if (shape->k_rows) {
-        const dim3 grid(key_tiles(a) * a.n_kv);
-#define FMLH_LAUNCH(DP) \
-    hipLaunchKernelGGL(attn_packed_dkv_kernel<DP>, grid, dim3(256), 0, stream(), a, dk, dv, ws, dout, lse, q, k, v)
-        FMLH_BY_DIM(FMLH_LAUNCH);
-#undef FMLH_LAUNCH
-        FMLH_LAUNCHED("attn_packed_dkv_kernel");
-    }
-    return FMLH_OK;
+    return attn_split_backward(a, shape->q_rows ? row_tiles(a, kRowsPerWG) : 0, shape->k_rows ? key_tiles(a) : 0, parts, dq, dk, dv, ws,
+                               dout, out, lse, q, k, v, ws + deltas(a), stream());
 }
 
 }  // extern "C"

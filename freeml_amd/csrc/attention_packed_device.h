@@ -166,19 +166,22 @@ __device__ __forceinline__ RowTile row_tile(const PackedAttn& a, const Work& w, 
     t.last = min(t.rho0 + per_tile, t.rows) - 1;
     t.shift = (int)w.sp.kl - (int)w.sp.ql;
     t.nkeys = min(t.last / a.group + t.shift + 1, (int)w.sp.kl);
-    t.k_begin = w.range * w.per;
-    t.k_end = min(t.nkeys - t.k_begin, w.per) + t.k_begin;
-    t.ranges = t.nkeys <= w.per ? 1 : (t.nkeys + w.per - 1) / w.per;
+    t.ranges = t.nkeys <= w.per ? 1 : (t.nkeys + w.per - 1) / w.per;  // of one length, about
+    const int each = t.ranges == 1 ? t.nkeys : ((t.nkeys + t.ranges - 1) / t.ranges + 63) / 64 * 64;
+    t.k_begin = w.range * each;
+    t.k_end = min(t.nkeys, t.k_begin + each);
     return t;
 }
 
-// Partial results of a tile's ranges in the workspace: maximum and sum of every row, then outputs.
+// Partial results of a tile's ranges in the workspace (16-byte aligned): outputs of every row, in whole
+// 16 bytes, then maxima and sums.
 struct Partials {
-    float *ml, *o;
+    float *o, *ml;
 };
+__host__ __device__ __forceinline__ int padded_dim(int dim) { return (dim + 3) & ~3; }
 __device__ __forceinline__ Partials partials(float* ws, uint32_t n_kv, uint32_t kv, uint32_t items, uint32_t item, int per_tile, int dim) {
     const size_t rows = (size_t)n_kv * items * per_tile, at = ((size_t)kv * items + item) * per_tile;
-    return Partials{ws + 2 * at, ws + 2 * rows + at * dim};
+    return Partials{ws + at * padded_dim(dim), ws + rows * padded_dim(dim) + 2 * at};
 }
 
 // Dims d .. d + 3 of a row, zeros past head_dim.

@@ -129,7 +129,21 @@ __device__ __forceinline__ floatx16 tile_product(const uintx4* planes, int row0,
     return s;
 }
 
-// acc (dims x 32 columns) += (tile rows row0 .. row0 + 31)^T times their weights w, w times 2^24.
+// acc (dims x 32 columns) += (tile rows row0 .. row0 + 15)^T times their weights x, x times 2^24.
+template <int R, int DP>
+__device__ __forceinline__ void tile_add16(floatx16 (&acc)[DP / 32], const uintx4* planes, int row0, const float (&x)[8], int lane) {
+    uintx4 u[3];
+    split8(x, u, kUp);
+#pragma unroll
+    for (int i = 0; i < DP / 32; ++i) {
+        bf16x8 a[3];
+#pragma unroll
+        for (int q = 0; q < 3; ++q) a[q] = column_operand<R, DP>(planes, q, row0, i, lane);
+#pragma unroll
+        for (int q = 0; q < 6; ++q)
+            acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[kSplitA[q]], __builtin_bit_cast(bf16x8, u[kSplitB[q]]), acc[i], 0, 0, 0);
+    }
+}
 template <int R, int DP>
 __device__ __forceinline__ void tile_add(floatx16 (&acc)[DP / 32], const uintx4* planes, int row0, const floatx16& w, int lane) {
 #pragma unroll
@@ -137,17 +151,7 @@ __device__ __forceinline__ void tile_add(floatx16 (&acc)[DP / 32], const uintx4*
         float x[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[e] = w[8 * t + e];
-        uintx4 u[3];
-        split8(x, u, kUp);
-#pragma unroll
-        for (int i = 0; i < DP / 32; ++i) {
-            bf16x8 a[3];
-#pragma unroll
-            for (int q = 0; q < 3; ++q) a[q] = column_operand<R, DP>(planes, q, row0 + 16 * t, i, lane);
-#pragma unroll
-            for (int q = 0; q < 6; ++q)
-                acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[kSplitA[q]], __builtin_bit_cast(bf16x8, u[kSplitB[q]]), acc[i], 0, 0, 0);
-        }
+        tile_add16<R, DP>(acc, planes, row0 + 16 * t, x, lane);
     }
 }
 
@@ -323,8 +327,8 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attn_split_kernel(Packe
         const int t = rho - tl.rho0;
         const Partials part = partials(ws, a.n_kv, kv, gridDim.x / a.n_kv, w.item0 + w.range, kRowsPerWG, dim);
         inv = 1.0f;
-        dst = part.o + t * dim;
-        dst_vec = false;
+        dst = part.o + t * padded_dim(dim);
+        dst_vec = true;
         if (h == 0) {
             part.ml[2 * t] = top;
             part.ml[2 * t + 1] = l;
@@ -345,7 +349,6 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attn_split_kernel(Packe
 
 // ---- backward --------------------------------------------------------------------------------
 
-// dq and d_i: tiles and lanes as in the forward pass; S^T = K Q^T, dP^T = V dO^T, dQ^T += K^T dS^T.
 // dq / scale of 32 rows again, from memory.
 template <int DP>
 __device__ __noinline__ void redo_dq(Redone<DP>& result, const PackedAttn& a, const float* kb, const float* vb, const float* q_row,
@@ -369,101 +372,6 @@ __device__ __noinline__ void redo_dq(Redone<DP>& result, const PackedAttn& a, co
     }
 #pragma unroll
     for (int i = 0; i < DP / 32; ++i) result.x[i] = acc[i];
-}
-
-template <int DP, bool VEC>
-__global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attn_split_dq_kernel(PackedAttn a, float* __restrict__ dq, float* __restrict__ delta,
-                                                               const float* __restrict__ dout, const float* __restrict__ out,
-                                                               const float* __restrict__ lse, const float* __restrict__ q,
-                                                               const float* __restrict__ k, const float* __restrict__ v) {
-    constexpr int KT = 32, U = DP / 8, NB = DP / 32;
-    __shared__ uintx4 kp[3 * KT * U];
-    __shared__ uintx4 vp[3 * KT * U];
-    const int kv = blockIdx.x % a.n_kv;
-    Work w;
-    if (!find_work<false, true>(a, kRowsPerWG, 0, blockIdx.x / a.n_kv, &w)) return;
-    const RowTile tl = row_tile(a, w, kRowsPerWG);
-    const Span sp = w.sp;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, c = lane & 31;
-    const int dim = a.head_dim, group = a.group, rows = tl.rows, shift = tl.shift, nkeys = tl.nkeys;
-    const bool vec = a.vec;
-    const int rho0 = tl.rho0 + wave * kRowsPerWave, rho = rho0 + c;
-    const bool live = rho < rows;
-    const int qi = (live ? rho : rows - 1) / group, head = kv * group + (live ? rho : rows - 1) % group;
-    const int limit = qi + shift;
-    const int first_limit = min(rho0, rows - 1) / group + shift;
-    const int last_limit = rho0 < rows ? (min(rho0 + kRowsPerWave, rows) - 1) / group + shift : -1;
-    const float* kb = k + (size_t)sp.k0 * a.k_rs + (size_t)kv * a.k_hs;
-    const float* vb = v + (size_t)sp.k0 * a.v_rs + (size_t)kv * a.v_hs;
-    const float* q_row = q + (size_t)(sp.q0 + qi) * a.q_rs + (size_t)head * dim;
-    const size_t o_at = (size_t)(sp.q0 + qi) * a.o_rs + (size_t)head * dim;
-    const float* g_row = dout + o_at;
-
-    Stage<KT, DP, VEC> ks, vs;
-    if (nkeys > 0) {
-        ks.load(kb, a.k_rs, 0, nkeys, dim);
-        vs.load(vb, a.v_rs, 0, nkeys, dim);
-    }
-    float d = 0.f;
-#pragma unroll
-    for (int st = 0; st < DP / 16; ++st)
-#pragma unroll
-        for (int e = 0; e < 8; e += 4) {
-            const floatx4 x = load4_padded<VEC>(g_row, 16 * st + 8 * h + e, dim, true),
-                          y = load4_padded<VEC>(out + o_at, 16 * st + 8 * h + e, dim, true);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) d += x[i] * y[i];
-        }
-    d += __shfl_xor(d, 32);
-    const size_t stat = (size_t)head * a.q_rows + sp.q0 + qi;
-    if (live && h == 0) delta[stat] = d;
-    const float lse2 = lse[stat] * kLog2e;
-    bf16x8 qp[3][DP / 16], gp[3][DP / 16];
-    load_operand<DP, VEC>(qp, q_row, h, dim);
-    load_operand<DP, VEC>(gp, g_row, h, dim);
-    floatx16 acc[NB];
-    clear(acc);
-    const float factor = a.scale * kLog2e;
-    for (int t0 = 0; t0 < nkeys; t0 += KT) {
-        lds_barrier();
-        ks.store(kp);
-        vs.store(vp);
-        if (t0 + KT < nkeys) {
-            ks.load(kb, a.k_rs, t0 + KT, nkeys, dim);
-            vs.load(vb, a.v_rs, t0 + KT, nkeys, dim);
-        }
-        lds_barrier();
-        if (t0 > last_limit) continue;
-        floatx16 s = tile_product<KT, DP>(kp, 0, qp, h, c);
-        const floatx16 dp = tile_product<KT, DP>(vp, 0, gp, h, c);
-        const bool edge = t0 + 31 > first_limit;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            const float x = fast_exp2(fmaf(s[r], factor * kDown2, -lse2)) * fmaf(dp[r], kDown2, -d);
-            s[r] = edge && t0 + acc_row(r, h) > limit ? 0.f : x;
-        }
-        tile_add<KT, DP>(acc, kp, 0, s, lane);
-    }
-    float unit = kDown2;
-    if (any_not_finite(acc)) {
-        unit = 1.0f;
-        Redone<DP> r;
-        redo_dq<DP>(r, a, kb, vb, q_row, g_row, lse2, d, nkeys, limit, last_limit);
-#pragma unroll
-        for (int i = 0; i < NB; ++i) acc[i] = r.x[i];
-    }
-    if (!live) return;
-    const float by = a.scale;
-    float* dst = dq + (size_t)(sp.q0 + qi) * a.q_rs + (size_t)head * dim;
-#pragma unroll
-    for (int i = 0; i < NB; ++i)
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            floatx4 x;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] = acc[i][4 * u + e] * unit * by;
-            store4(dst, 32 * i + 8 * u + 4 * h, dim, vec, x);
-        }
 }
 
 // The two waves of a pair hand 32 x 32 values to one another through LDS as their accumulators lie.
@@ -518,26 +426,142 @@ __device__ __noinline__ void redo_dkv(Redone<DP>& result, const PackedAttn& a, c
     for (int i = 0; i < DP / 32; ++i) result.x[i] = acc[i];
 }
 
+// Tiles of the backward pass: 64 rows or keys in LDS at head_dim 33 .. 64, else 32 (LDS at 128 would hold no more;
+// at 32 it leaves room for two work-groups).
+template <int DP>
+constexpr int kBackTile = DP == 64 ? 64 : 32;
+
+template <int DP>
+struct BackwardLds {
+    static constexpr int T = kBackTile<DP>;
+    uintx4 planes[2][3 * T * (DP / 8)];
+    Exchange exchange[T / 32][4];
+    __attribute__((aligned(16))) float stats[2][T];
+};
+
+// dq of 128 rows, two waves for each 32 of them (as in the forward pass a row per lane column):
+//   the first S^T = K Q^T and p, the second dP^T = V dO^T - d; each hands half of its keys' values to the
+// other, forms dS of the other half and adds K^T dS over it: dQ^T is the sum of the two.
+template <int DP, bool VEC>
+__device__ __forceinline__ void dq_tile(BackwardLds<DP>& lds, const PackedAttn& a, uint32_t index, float* __restrict__ dq,
+                                        const float* __restrict__ delta, const float* __restrict__ dout, const float* __restrict__ lse,
+                                        const float* __restrict__ q, const float* __restrict__ k, const float* __restrict__ v) {
+    constexpr int KT = kBackTile<DP>, NB = DP / 32;
+    const int kv = index % a.n_kv;
+    Work w;
+    if (!find_work<false, true>(a, kRowsPerWG, 0, index / a.n_kv, &w)) return;
+    const RowTile tl = row_tile(a, w, kRowsPerWG);
+    const Span sp = w.sp;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, c = lane & 31;
+    const int pair = wave & 3, second = wave >> 2;
+    const int dim = a.head_dim, group = a.group, rows = tl.rows, shift = tl.shift, nkeys = tl.nkeys;
+    const int rho0 = tl.rho0 + pair * kRowsPerWave, rho = rho0 + c;
+    const bool live = rho < rows;
+    const int qi = (live ? rho : rows - 1) / group, head = kv * group + (live ? rho : rows - 1) % group;
+    const int limit = qi + shift;
+    const int first_limit = min(rho0, rows - 1) / group + shift;
+    const int last_limit = rho0 < rows ? (min(rho0 + kRowsPerWave, rows) - 1) / group + shift : -1;
+    const float* kb = k + (size_t)sp.k0 * a.k_rs + (size_t)kv * a.k_hs;
+    const float* vb = v + (size_t)sp.k0 * a.v_rs + (size_t)kv * a.v_hs;
+    const float* q_row = q + (size_t)(sp.q0 + qi) * a.q_rs + (size_t)head * dim;
+    const float* g_row = dout + (size_t)(sp.q0 + qi) * a.o_rs + (size_t)head * dim;
+
+    // The first four waves stage K, the others V.
+    Stage<KT, DP, VEC> keys;
+    const float* const base = second ? vb : kb;
+    const size_t rs = second ? a.v_rs : a.k_rs;
+    if (nkeys > 0) keys.load(base, rs, 0, nkeys, dim);
+    const size_t stat = (size_t)head * a.q_rows + sp.q0 + qi;
+    const float lse2 = lse[stat] * kLog2e, d = delta[stat];
+    bf16x8 own[3][DP / 16];  // Q's, dO's parts
+    load_operand<DP, VEC>(own, second ? g_row : q_row, h, dim);
+    floatx16 acc[NB];
+    clear(acc);
+    const float factor = a.scale * kLog2e;
+    for (int t0 = 0; t0 < nkeys; t0 += KT) {
+        lds_barrier();
+        keys.store(lds.planes[second]);
+        if (t0 + KT < nkeys) keys.load(base, rs, t0 + KT, nkeys, dim);
+        lds_barrier();
+        floatx16 s[KT / 32];
+#pragma unroll
+        for (int j = 0; j < KT / 32; ++j) {
+            if (t0 + 32 * j > last_limit) continue;  // no row of the wave sees the block
+            s[j] = tile_product<KT, DP>(lds.planes[second], 32 * j, own, h, c);
+            const bool edge = t0 + 32 * j + 31 > first_limit;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const float x = second ? fmaf(s[j][r], kDown2, -d) : fast_exp2(fmaf(s[j][r], factor * kDown2, -lse2));
+                s[j][r] = edge && t0 + 32 * j + acc_row(r, h) > limit ? 0.f : x;
+            }
+            Exchange& ex = lds.exchange[j][pair];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                ex.x[2 * second + u][lane] = second ? floatx4{s[j][4 * u], s[j][4 * u + 1], s[j][4 * u + 2], s[j][4 * u + 3]}
+                                                    : floatx4{s[j][4 * u + 8], s[j][4 * u + 9], s[j][4 * u + 10], s[j][4 * u + 11]};
+            }
+        }
+        lds_barrier();
+#pragma unroll
+        for (int j = 0; j < KT / 32; ++j) {
+            if (t0 + 32 * j > last_limit) continue;
+            const Exchange& ex = lds.exchange[j][pair];
+            const floatx4 y0 = ex.x[2 - 2 * second][lane], y1 = ex.x[3 - 2 * second][lane];
+            float x[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = (second ? s[j][8 + e] : s[j][e]) * (e < 4 ? y0[e & 3] : y1[e & 3]);
+            tile_add16<KT, DP>(acc, lds.planes[0], 32 * j + 16 * second, x, lane);
+        }
+    }
+    // The second waves' sums, a block of 32 dims at a time.
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+        lds_barrier();
+        if (second) lds.exchange[0][pair].put(acc[i], lane);
+        lds_barrier();
+        if (!second) acc[i] += lds.exchange[0][pair].get(lane);
+    }
+    if (second) return;
+    float unit = kDown2;
+    if (any_not_finite(acc)) {
+        unit = 1.0f;
+        Redone<DP> r;
+        redo_dq<DP>(r, a, kb, vb, q_row, g_row, lse2, d, nkeys, limit, last_limit);
+#pragma unroll
+        for (int i = 0; i < NB; ++i) acc[i] = r.x[i];
+    }
+    if (!live) return;
+    float* dst = dq + (size_t)(sp.q0 + qi) * a.q_rs + (size_t)head * dim;
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            floatx4 x;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = acc[i][4 * u + e] * unit * a.scale;
+            store4(dst, 32 * i + 8 * u + 4 * h, dim, a.vec, x);
+        }
+}
+
 // dk and dv: a work-group per 128 keys of one (sequence, key head), a key per lane column; the rows of
 // the group's heads stream through LDS.  Two waves share 32 keys (keeping K and V parts and both sums
 // in one wave's registers spilled at head_dim 128: 4.9 ms where this takes @DKV128@):
 //   the first   S = Q K^T, p, dV^T += dO^T P     holds K and dV,
 //   the second  dP = dO V^T, dS, dK^T += Q^T dS  holds V and dK and takes p from the first.
-// Where there are few such tiles, their rows are cut into gridDim.y parts (whole tiles of rows, of
-// all heads in order); the parts' sums go to the workspace and attn_split_dkv_join_kernel adds them in order.
+// Where there are few such tiles, their rows are cut into parts (whole tiles of rows, of all heads in
+// order); the parts' sums go to the workspace and attn_split_dkv_join_kernel adds them in order.
 template <int DP, bool VEC>
-__global__ __launch_bounds__(512, DP == 32 ? 4 : 2) void attn_split_dkv_kernel(PackedAttn a, float* __restrict__ dk, float* __restrict__ dv,
-                                                                const float* __restrict__ delta, const float* __restrict__ dout,
-                                                                const float* __restrict__ lse, const float* __restrict__ q,
-                                                                const float* __restrict__ k, const float* __restrict__ v,
-                                                                float* __restrict__ part) {
-    constexpr int RT = DP == 64 ? 64 : 32, U = DP / 8, NB = DP / 32;
-    __shared__ uintx4 planes[2][3 * RT * U];  // Q, dO
-    __shared__ Exchange exchange[RT / 32][4];
-    __shared__ __attribute__((aligned(16))) float stats[2][RT];  // lse (base 2), d
-    const int kv = blockIdx.x % a.n_kv;
+__device__ __forceinline__ void dkv_tile(BackwardLds<DP>& lds, const PackedAttn& a, uint32_t index, uint32_t tiles_all, int part, int parts,
+                                         float* __restrict__ dk, float* __restrict__ dv, const float* __restrict__ delta,
+                                         const float* __restrict__ dout, const float* __restrict__ lse, const float* __restrict__ q,
+                                         const float* __restrict__ k, const float* __restrict__ v, float* __restrict__ sums) {
+    constexpr int RT = kBackTile<DP>, NB = DP / 32;
+    auto& planes = lds.planes;      // Q, dO
+    auto& exchange = lds.exchange;
+    auto& stats = lds.stats;        // lse (base 2), d
+    const int kv = index % a.n_kv;
     Work w;
-    if (!find_work<true, true>(a, kRowsPerWG, 0, blockIdx.x / a.n_kv, &w)) return;
+    if (!find_work<true, true>(a, kRowsPerWG, 0, index / a.n_kv, &w)) return;
     const Span sp = w.sp;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, c = lane & 31;
     const int pair = wave & 3, second = wave >> 2;
@@ -552,7 +576,7 @@ __global__ __launch_bounds__(512, DP == 32 ? 4 : 2) void attn_split_dkv_kernel(P
     // The tiles of rows that see a key of the work-group, over the group's heads, and this part of them.
     const int first = max(0, (int)w.tile * kRowsPerWG - shift) / RT, tiles = max(0, (ql + RT - 1) / RT - first);
     const int64_t total = (int64_t)tiles * group;
-    const int it0 = (int)(total * blockIdx.y / gridDim.y), it1 = (int)(total * (blockIdx.y + 1) / gridDim.y);
+    const int it0 = (int)(total * part / parts), it1 = (int)(total * (part + 1) / parts);
 
     bf16x8 own[3][DP / 16];  // K's, V's parts
     load_operand<DP, VEC>(own, second ? v_row : k_row, h, dim);
@@ -632,9 +656,9 @@ __global__ __launch_bounds__(512, DP == 32 ? 4 : 2) void attn_split_dkv_kernel(P
     float* dst = second ? dk + row * a.k_rs + (size_t)kv * a.k_hs : dv + row * a.v_rs + (size_t)kv * a.v_hs;
     bool dst_vec = vec;
     int width = dim;
-    if (gridDim.y > 1) {
-        const size_t tile = (size_t)blockIdx.y * gridDim.x + (size_t)w.tile0 * a.n_kv + kv;
-        dst = part + ((tile * 2 + 1 - second) * kRowsPerWG + key - w.tile * kRowsPerWG) * DP;
+    if (parts > 1) {
+        const size_t tile = (size_t)part * tiles_all + (size_t)w.tile0 * a.n_kv + kv;
+        dst = sums + ((tile * 2 + 1 - second) * kRowsPerWG + key - w.tile * kRowsPerWG) * DP;
         dst_vec = true;
         width = DP;
     }
@@ -648,6 +672,41 @@ __global__ __launch_bounds__(512, DP == 32 ? 4 : 2) void attn_split_dkv_kernel(P
             for (int e = 0; e < 4; ++e) x[e] = acc[i][4 * u + e] * unit * by;
             store4(dst, 32 * i + 8 * u + 4 * h, width, dst_vec, x);
         }
+}
+
+// The backward pass in one launch: the tiles of dk and dv first (they take longest), then those of dq,
+// which need nothing of them.
+template <int DP, bool VEC>
+__global__ __launch_bounds__(512, DP == 32 ? 4 : 2) void attn_split_backward_kernel(
+    PackedAttn a, uint32_t key_groups, int parts, float* __restrict__ dq, float* __restrict__ dk, float* __restrict__ dv,
+    const float* __restrict__ delta, const float* __restrict__ dout, const float* __restrict__ lse, const float* __restrict__ q,
+    const float* __restrict__ k, const float* __restrict__ v, float* __restrict__ sums) {
+    __shared__ BackwardLds<DP> lds;
+    if (blockIdx.x < key_groups * parts)
+        dkv_tile<DP, VEC>(lds, a, blockIdx.x % key_groups, key_groups, blockIdx.x / key_groups, parts, dk, dv, delta, dout, lse, q, k, v, sums);
+    else
+        dq_tile<DP, VEC>(lds, a, blockIdx.x - key_groups * parts, dq, delta, dout, lse, q, k, v);
+}
+
+// d_i = do_i . o_i of every row and head: LPR lanes each.
+template <int LPR>
+__global__ __launch_bounds__(256) void attn_split_delta_kernel(PackedAttn a, float* __restrict__ delta, const float* __restrict__ dout,
+                                                               const float* __restrict__ out) {
+    const uint32_t heads = a.n_kv * a.group, lane = threadIdx.x % LPR;
+    const uint64_t i = ((uint64_t)blockIdx.x * 256 + threadIdx.x) / LPR;
+    const uint32_t row = (uint32_t)(i / heads), head = (uint32_t)(i % heads);
+    float d = 0.f;
+    if (row < a.q_rows) {
+        const size_t at = (size_t)row * a.o_rs + (size_t)head * a.head_dim;
+        for (int e = 4 * lane; e < a.head_dim; e += 4 * LPR) {
+            const floatx4 x = load4(dout + at, e, a.head_dim, a.vec), y = load4(out + at, e, a.head_dim, a.vec);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) d += x[j] * y[j];
+        }
+    }
+#pragma unroll
+    for (int m = 1; m < LPR; m <<= 1) d += __shfl_xor(d, m);
+    if (row < a.q_rows && lane == 0) delta[(size_t)head * a.q_rows + row] = d;
 }
 
 // dk and dv of a tile of keys: its parts added in order.
@@ -692,31 +751,30 @@ int attn_split_forward(const PackedAttn& a, uint32_t items, uint32_t budget, flo
     return FMLH_OK;
 }
 
-int attn_split_dq(const PackedAttn& a, uint32_t tiles, float* dq, float* delta, const float* dout, const float* out, const float* lse,
-                  const float* q, const float* k, const float* v, hipStream_t s) {
-    const dim3 grid(tiles * a.n_kv);
-#define FMLH_LAUNCH(DP) hipLaunchKernelGGL((a.vec ? attn_split_dq_kernel<DP, true> : attn_split_dq_kernel<DP, false>), grid, dim3(256), 0, s, a, dq, delta, dout, out, lse, q, k, v)
-    FMLH_BY_DIM(FMLH_LAUNCH);
-#undef FMLH_LAUNCH
-    FMLH_LAUNCHED("attn_split_dq_kernel");
-    return FMLH_OK;
-}
-
 size_t attn_split_part_floats(const PackedAttn& a, uint32_t tiles) {
     const size_t dp = a.head_dim <= 32 ? 32 : a.head_dim <= 64 ? 64 : a.head_dim <= 96 ? 96 : 128;
     return (size_t)tiles * a.n_kv * 2 * kRowsPerWG * dp;
 }
 
-int attn_split_dkv(const PackedAttn& a, uint32_t tiles, int parts, float* dk, float* dv, const float* delta, const float* dout,
-                   const float* lse, const float* q, const float* k, const float* v, float* part, hipStream_t s) {
-    const dim3 grid(tiles * a.n_kv, parts);
-#define FMLH_LAUNCH(DP) \
-    hipLaunchKernelGGL((a.vec ? attn_split_dkv_kernel<DP, true> : attn_split_dkv_kernel<DP, false>), grid, dim3(512), 0, s, a, dk, dv, delta, dout, lse, q, k, v, part)
+int attn_split_backward(const PackedAttn& a, uint32_t row_tiles, uint32_t key_tiles, int parts, float* dq, float* dk, float* dv,
+                        float* delta, const float* dout, const float* out, const float* lse, const float* q, const float* k,
+                        const float* v, float* sums, hipStream_t s) {
+    constexpr int kLanes = 16;
+    const uint64_t items = (uint64_t)a.q_rows * a.n_kv * a.group;
+    if (items) {
+        hipLaunchKernelGGL(attn_split_delta_kernel<kLanes>, dim3((unsigned)((items * kLanes + 255) / 256)), dim3(256), 0, s, a, delta, dout, out);
+        FMLH_LAUNCHED("attn_split_delta_kernel");
+    }
+    const uint32_t key_groups = key_tiles * a.n_kv;
+    const dim3 grid(key_groups * parts + row_tiles * a.n_kv);
+#define FMLH_LAUNCH(DP)                                                                                                               \
+    hipLaunchKernelGGL((a.vec ? attn_split_backward_kernel<DP, true> : attn_split_backward_kernel<DP, false>), grid, dim3(512), 0, s, a, \
+                       key_groups, parts, dq, dk, dv, delta, dout, lse, q, k, v, sums)
     FMLH_BY_DIM(FMLH_LAUNCH);
 #undef FMLH_LAUNCH
-    FMLH_LAUNCHED("attn_split_dkv_kernel");
+    FMLH_LAUNCHED("attn_split_backward_kernel");
     if (parts > 1) {
-#define FMLH_LAUNCH(DP) hipLaunchKernelGGL(attn_split_dkv_join_kernel<DP>, dim3(grid.x, 8), dim3(256), 0, s, a, dk, dv, part, parts)
+#define FMLH_LAUNCH(DP) hipLaunchKernelGGL(attn_split_dkv_join_kernel<DP>, dim3(key_groups, 8), dim3(256), 0, s, a, dk, dv, sums, parts)
         FMLH_BY_DIM(FMLH_LAUNCH);
 #undef FMLH_LAUNCH
         FMLH_LAUNCHED("attn_split_dkv_join_kernel");

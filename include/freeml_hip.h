@@ -279,7 +279,7 @@ typedef struct fmlh_packed_attention {
     uint32_t n_seq;
     uint32_t q_rows, k_rows; /* rows that exist; offsets beyond them are cut */
     uint32_t n_head, n_kv_head, head_dim;
-    float scale; /* usually 1 / sqrt(head_dim) */
+    float scale; /* usually 1 / sqrt(head_dim); 0 or of 2^-60 .. 2^60 */
     const int32_t* q_off; /* n_seq + 1 */
     const int32_t* k_off; /* n_seq + 1 */
     const int32_t* k_len; /* n_seq, or NULL */
@@ -288,7 +288,7 @@ typedef struct fmlh_packed_attention {
 } fmlh_packed_attention;
 
 /* Floats of device workspace that a forward call of this shape needs (backward = 0; 0 floats: none),
- * or enough for the forward and the backward call (backward = 1).  It depends on the sizes alone, not on the offsets' contents.  A workspace serves one call
+ * or enough for the forward and the backward call (backward = 1); 16-byte aligned.  It depends on the sizes alone, not on the offsets' contents.  A workspace serves one call
  * at a time: calls and captured graphs that may run at once need one each. */
 int fmlh_attention_packed_workspace(const fmlh_packed_attention* shape, int backward, size_t* floats);
 

@@ -451,7 +451,7 @@ def shape(**over):
 
 BAD = [dict(n_head=0), dict(n_kv_head=0), dict(n_head=5), dict(head_dim=0), dict(head_dim=129), dict(q_off=None), dict(k_off=None),
        dict(q_rs=31), dict(o_rs=8), dict(k_rs=7), dict(v_rs=7), dict(k_hs=7), dict(v_hs=1), dict(scale=float("nan")),
-       dict(scale=float("inf")), dict(q_rows=2**30 + 1), dict(k_rows=2**31), dict(n_seq=2**22 + 1), dict(q_rows=2**30, n_kv_head=1),
+       dict(scale=float("inf")), dict(scale=1e-19), dict(scale=-1e19), dict(q_rows=2**30 + 1), dict(k_rows=2**31), dict(n_seq=2**22 + 1), dict(q_rows=2**30, n_kv_head=1),
        dict(q_rs=2**32), dict(n_head=65536, n_kv_head=65536, q_rs=2**20, o_rs=2**20)]
 
 
