@@ -20,6 +20,9 @@ struct PackedAttn {
 // key head; ws, delta and sums are workspace.
 int attn_split_forward(const PackedAttn& a, uint32_t items, uint32_t budget, float* out, float* lse, const float* q, const float* k,
                        const float* v, float* ws, hipStream_t s);
+// Rows, or keys, of a tile of the backward pass.
+int attn_split_dq_rows(const PackedAttn& a);
+int attn_split_back_rows(const PackedAttn& a);
 // Floats that one of the parts of dk and dv leaves in `sums` (parts > 1).
 size_t attn_split_part_floats(const PackedAttn& a, uint32_t key_tiles);
 int attn_split_backward(const PackedAttn& a, uint32_t row_tiles, uint32_t key_tiles, int parts, float* dq, float* dk, float* dv,

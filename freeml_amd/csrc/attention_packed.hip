@@ -290,7 +290,7 @@ PackedAttn make_args(const fmlh_packed_attention* s) {
 }
 
 uint32_t row_tiles(const PackedAttn& a, uint32_t per) { return (uint32_t)(((uint64_t)a.q_rows * a.group) / per) + a.n_seq; }
-uint32_t key_tiles(const PackedAttn& a) { return a.k_rows / kRowsPerWG + a.n_seq; }
+uint32_t key_tiles(const PackedAttn& a) { return a.k_rows / attn_split_back_rows(a) + a.n_seq; }
 
 // Sequences of fewer keys are not cut: joining the ranges costs a launch of 5 us.
 constexpr uint64_t kCutKeys = 512;
@@ -325,7 +325,7 @@ constexpr uint64_t kMaxGroups = 1u << 23;
 
 // How the backward pass cuts the rows that a tile of keys sees.
 int plan_parts(const PackedAttn& a) {
-    const uint64_t tiles = std::max<uint64_t>(std::min(a.n_seq, key_tiles(a)), a.k_rows / kRowsPerWG) * a.n_kv;
+    const uint64_t tiles = std::max<uint64_t>(a.n_seq, a.k_rows / attn_split_back_rows(a)) * a.n_kv;
     const uint64_t want = 1024;          // work-groups that keep the device busy although early keys see more rows than late ones
     const size_t most = size_t(1) << 26;  // floats of partial sums
     const uint64_t fit = std::max<uint64_t>(1, most / std::max<size_t>(1, attn_split_part_floats(a, key_tiles(a))));
@@ -427,13 +427,13 @@ int fmlh_attention_packed_backward(const fmlh_packed_attention* shape, float* dq
     const int parts = plan_parts(a);
     const size_t need = deltas(a) + (parts > 1 ? parts * attn_split_part_floats(a, key_tiles(a)) : 0);
     FMLH_REQUIRE(need == 0 || (ws && ws_floats >= need), "%s: a workspace of %zu floats is needed", fn, need);
-    FMLH_REQUIRE(((uint64_t)row_tiles(a, kRowsPerWG) + (uint64_t)key_tiles(a) * parts) * a.n_kv <= kMaxGroups / 2 &&
+    FMLH_REQUIRE(((uint64_t)row_tiles(a, attn_split_dq_rows(a)) + (uint64_t)key_tiles(a) * parts) * a.n_kv <= kMaxGroups / 2 &&
                      (uint64_t)a.q_rows * shape->n_head <= (uint64_t(1) << 27),
                  "%s: more than 2^22 tiles of rows and keys, or 2^27 rows of heads", fn);
     a.vec = a.vec && aligned16(q) && aligned16(k) && aligned16(v) && aligned16(out) && aligned16(dout) && aligned16(dq) &&
             aligned16(dk) && aligned16(dv);
     FMLH_REQUIRE((uintptr_t)ws % 16 == 0, "%s: the workspace is not 16-byte aligned", fn);
-    return attn_split_backward(a, shape->q_rows ? row_tiles(a, kRowsPerWG) : 0, shape->k_rows ? key_tiles(a) : 0, parts, dq, dk, dv, ws,
+    return attn_split_backward(a, shape->q_rows ? row_tiles(a, attn_split_dq_rows(a)) : 0, shape->k_rows ? key_tiles(a) : 0, parts, dq, dk, dv, ws,
                                dout, out, lse, q, k, v, ws + deltas(a), stream());
 }
 

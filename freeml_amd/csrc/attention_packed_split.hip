@@ -32,19 +32,19 @@ struct Shape {
     __device__ static __forceinline__ int swz(int r) { return U % 8 == 0 ? (r & 7) : ((r >> 2) & 3); }
 };
 
-// R rows of a matrix in the registers of 256 threads (a thread's share) and from there as planes in LDS.
-template <int R, int DP, bool VEC>
+// R rows of a matrix in the registers of NT threads (a thread's share) and from there as planes in LDS.
+template <int R, int DP, bool VEC, int NT = 256>
 struct Stage {
-    static constexpr int U = DP / 8, N = (R * U + 255) / 256;
+    static constexpr int U = DP / 8, N = (R * U + NT - 1) / NT;
     floatx4 x[N][2];
     // Rows first .. of a matrix at base (64-bit, uniform), row stride rs; rows from `rows` on (rows > first) are zeros.
     __device__ __forceinline__ void load(const float* base, size_t rs, int first, int rows, int dim) {
-        const int t = threadIdx.x & 255;
+        const int t = threadIdx.x & (NT - 1);
         const float* tile = base + (size_t)first * rs;
-        if (VEC && R * U % 256 == 0 && first + R <= rows && dim == DP) {
+        if (VEC && R * U % NT == 0 && first + R <= rows && dim == DP) {
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                const int u = t + 256 * i;
+                const int u = t + NT * i;
                 const floatx4* row = reinterpret_cast<const floatx4*>(tile + (size_t)(u / U) * rs + 8 * (u % U));
                 x[i][0] = row[0];
                 x[i][1] = row[1];
@@ -53,7 +53,7 @@ struct Stage {
         }
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int u = min(t + 256 * i, R * U - 1), r = u / U, d = 8 * (u % U);
+            const int u = min(t + NT * i, R * U - 1), r = u / U, d = 8 * (u % U);
             const bool on = first + r < rows;
             const float* row = tile + (size_t)(on ? r : 0) * rs;
             x[i][0] = load4_padded<VEC>(row, d, dim, on);
@@ -63,8 +63,8 @@ struct Stage {
     __device__ __forceinline__ void store(uintx4* planes) const {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int u = (threadIdx.x & 255) + 256 * i, r = u / U;
-            if (R * U % 256 != 0 && u >= R * U) break;
+            const int u = (threadIdx.x & (NT - 1)) + NT * i, r = u / U;
+            if (R * U % NT != 0 && u >= R * U) break;
             const float v[8] = {x[i][0][0], x[i][0][1], x[i][0][2], x[i][0][3], x[i][1][0], x[i][1][1], x[i][1][2], x[i][1][3]};
             uintx4 p[3];
             split8(v, p, kUp);
@@ -426,34 +426,41 @@ __device__ __noinline__ void redo_dkv(Redone<DP>& result, const PackedAttn& a, c
     for (int i = 0; i < DP / 32; ++i) result.x[i] = acc[i];
 }
 
+// Keys of a sequence from which on a work-group of the backward pass has four pairs of waves.
+#ifndef PBIG
+#define PBIG 4
+#endif
+constexpr uint32_t kLongKeys = 1536;
+
 // Tiles of the backward pass: 64 rows or keys in LDS at head_dim 33 .. 64, else 32 (LDS at 128 would hold no more;
 // at 32 it leaves room for two work-groups).
 template <int DP>
 constexpr int kBackTile = DP == 64 ? 64 : 32;
 
-template <int DP>
+// P: pairs of waves per work-group.
+template <int DP, int P>
 struct BackwardLds {
     static constexpr int T = kBackTile<DP>;
     uintx4 planes[2][3 * T * (DP / 8)];
-    Exchange exchange[T / 32][4];
+    Exchange exchange[T / 32][P];
     __attribute__((aligned(16))) float stats[2][T];
 };
 
-// dq of 128 rows, two waves for each 32 of them (as in the forward pass a row per lane column):
+// dq of a tile of rows, two waves for each 32 of them (as in the forward pass a row per lane column):
 //   the first S^T = K Q^T and p, the second dP^T = V dO^T - d; each hands half of its keys' values to the
 // other, forms dS of the other half and adds K^T dS over it: dQ^T is the sum of the two.
-template <int DP, bool VEC>
-__device__ __forceinline__ void dq_tile(BackwardLds<DP>& lds, const PackedAttn& a, uint32_t index, float* __restrict__ dq,
+template <int DP, bool VEC, int P>
+__device__ __forceinline__ void dq_tile(BackwardLds<DP, P>& lds, const PackedAttn& a, uint32_t index, float* __restrict__ dq,
                                         const float* __restrict__ delta, const float* __restrict__ dout, const float* __restrict__ lse,
                                         const float* __restrict__ q, const float* __restrict__ k, const float* __restrict__ v) {
-    constexpr int KT = kBackTile<DP>, NB = DP / 32;
+    constexpr int KT = kBackTile<DP>, NB = DP / 32, kTile = 32 * P;
     const int kv = index % a.n_kv;
     Work w;
-    if (!find_work<false, true>(a, kRowsPerWG, 0, index / a.n_kv, &w)) return;
-    const RowTile tl = row_tile(a, w, kRowsPerWG);
+    if (!find_work<false, true>(a, kTile, 0, index / a.n_kv, &w)) return;
+    const RowTile tl = row_tile(a, w, kTile);
     const Span sp = w.sp;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, c = lane & 31;
-    const int pair = wave & 3, second = wave >> 2;
+    const int pair = wave % P, second = wave / P;
     const int dim = a.head_dim, group = a.group, rows = tl.rows, shift = tl.shift, nkeys = tl.nkeys;
     const int rho0 = tl.rho0 + pair * kRowsPerWave, rho = rho0 + c;
     const bool live = rho < rows;
@@ -466,8 +473,8 @@ __device__ __forceinline__ void dq_tile(BackwardLds<DP>& lds, const PackedAttn& 
     const float* q_row = q + (size_t)(sp.q0 + qi) * a.q_rs + (size_t)head * dim;
     const float* g_row = dout + (size_t)(sp.q0 + qi) * a.o_rs + (size_t)head * dim;
 
-    // The first four waves stage K, the others V.
-    Stage<KT, DP, VEC> keys;
+    // The first waves stage K, the others V.
+    Stage<KT, DP, VEC, 64 * P> keys;
     const float* const base = second ? vb : kb;
     const size_t rs = second ? a.v_rs : a.k_rs;
     if (nkeys > 0) keys.load(base, rs, 0, nkeys, dim);
@@ -543,38 +550,117 @@ __device__ __forceinline__ void dq_tile(BackwardLds<DP>& lds, const PackedAttn& 
         }
 }
 
-// dk and dv: a work-group per 128 keys of one (sequence, key head), a key per lane column; the rows of
+// dq of a tile of rows, a wave for each 32 of them, as in the forward pass: S^T = K Q^T, dP^T = V dO^T,
+// dQ^T += K^T dS^T.
+template <int DP, bool VEC, int P>
+__device__ __forceinline__ void dq_tile_alone(BackwardLds<DP, P>& lds, const PackedAttn& a, uint32_t index, float* __restrict__ dq,
+                                              const float* __restrict__ delta, const float* __restrict__ dout, const float* __restrict__ lse,
+                                              const float* __restrict__ q, const float* __restrict__ k, const float* __restrict__ v) {
+    constexpr int KT = kBackTile<DP>, NB = DP / 32, kTile = 64 * P, NT = 64 * P;
+    const int kv = index % a.n_kv;
+    Work w;
+    if (!find_work<false, true>(a, kTile, 0, index / a.n_kv, &w)) return;
+    const RowTile tl = row_tile(a, w, kTile);
+    const Span sp = w.sp;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, c = lane & 31;
+    const int second = wave / P;
+    const int dim = a.head_dim, group = a.group, rows = tl.rows, shift = tl.shift, nkeys = tl.nkeys;
+    const int rho0 = tl.rho0 + wave * kRowsPerWave, rho = rho0 + c;
+    const bool live = rho < rows;
+    const int qi = (live ? rho : rows - 1) / group, head = kv * group + (live ? rho : rows - 1) % group;
+    const int limit = qi + shift;
+    const int first_limit = min(rho0, rows - 1) / group + shift;
+    const int last_limit = rho0 < rows ? (min(rho0 + kRowsPerWave, rows) - 1) / group + shift : -1;
+    const float* kb = k + (size_t)sp.k0 * a.k_rs + (size_t)kv * a.k_hs;
+    const float* vb = v + (size_t)sp.k0 * a.v_rs + (size_t)kv * a.v_hs;
+    const float* q_row = q + (size_t)(sp.q0 + qi) * a.q_rs + (size_t)head * dim;
+    const float* g_row = dout + (size_t)(sp.q0 + qi) * a.o_rs + (size_t)head * dim;
+
+    // The first waves stage K, the others V.
+    Stage<KT, DP, VEC, NT> keys;
+    const float* const base = second ? vb : kb;
+    const size_t rs = second ? a.v_rs : a.k_rs;
+    if (nkeys > 0) keys.load(base, rs, 0, nkeys, dim);
+    const size_t stat = (size_t)head * a.q_rows + sp.q0 + qi;
+    const float lse2 = lse[stat] * kLog2e, d = delta[stat];
+    bf16x8 qp[3][DP / 16], gp[3][DP / 16];
+    load_operand<DP, VEC>(qp, q_row, h, dim);
+    load_operand<DP, VEC>(gp, g_row, h, dim);
+    floatx16 acc[NB];
+    clear(acc);
+    const float factor = a.scale * kLog2e;
+    for (int t0 = 0; t0 < nkeys; t0 += KT) {
+        lds_barrier();
+        keys.store(lds.planes[second]);
+        if (t0 + KT < nkeys) keys.load(base, rs, t0 + KT, nkeys, dim);
+        lds_barrier();
+#pragma unroll
+        for (int j = 0; j < KT / 32; ++j) {
+            if (t0 + 32 * j > last_limit) continue;  // no row of the wave sees the block
+            floatx16 s = tile_product<KT, DP>(lds.planes[0], 32 * j, qp, h, c);
+            const floatx16 dp = tile_product<KT, DP>(lds.planes[1], 32 * j, gp, h, c);
+            const bool edge = t0 + 32 * j + 31 > first_limit;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const float x = fast_exp2(fmaf(s[r], factor * kDown2, -lse2)) * fmaf(dp[r], kDown2, -d);
+                s[r] = edge && t0 + 32 * j + acc_row(r, h) > limit ? 0.f : x;
+            }
+            tile_add<KT, DP>(acc, lds.planes[0], 32 * j, s, lane);
+        }
+    }
+    float unit = kDown2;
+    if (any_not_finite(acc)) {
+        unit = 1.0f;
+        Redone<DP> r;
+        redo_dq<DP>(r, a, kb, vb, q_row, g_row, lse2, d, nkeys, limit, last_limit);
+#pragma unroll
+        for (int i = 0; i < NB; ++i) acc[i] = r.x[i];
+    }
+    if (!live) return;
+    float* dst = dq + (size_t)(sp.q0 + qi) * a.q_rs + (size_t)head * dim;
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            floatx4 x;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = acc[i][4 * u + e] * unit * a.scale;
+            store4(dst, 32 * i + 8 * u + 4 * h, dim, a.vec, x);
+        }
+}
+
+// dk and dv: a work-group per tile of keys of one (sequence, key head), a key per lane column; the rows of
 // the group's heads stream through LDS.  Two waves share 32 keys (keeping K and V parts and both sums
 // in one wave's registers spilled at head_dim 128: 4.9 ms where this takes @DKV128@):
 //   the first   S = Q K^T, p, dV^T += dO^T P     holds K and dV,
 //   the second  dP = dO V^T, dS, dK^T += Q^T dS  holds V and dK and takes p from the first.
 // Where there are few such tiles, their rows are cut into parts (whole tiles of rows, of all heads in
 // order); the parts' sums go to the workspace and attn_split_dkv_join_kernel adds them in order.
-template <int DP, bool VEC>
-__device__ __forceinline__ void dkv_tile(BackwardLds<DP>& lds, const PackedAttn& a, uint32_t index, uint32_t tiles_all, int part, int parts,
+template <int DP, bool VEC, int P>
+__device__ __forceinline__ void dkv_tile(BackwardLds<DP, P>& lds, const PackedAttn& a, uint32_t index, uint32_t tiles_all, int part, int parts,
                                          float* __restrict__ dk, float* __restrict__ dv, const float* __restrict__ delta,
                                          const float* __restrict__ dout, const float* __restrict__ lse, const float* __restrict__ q,
                                          const float* __restrict__ k, const float* __restrict__ v, float* __restrict__ sums) {
-    constexpr int RT = kBackTile<DP>, NB = DP / 32;
+    constexpr int RT = kBackTile<DP>, NB = DP / 32, kTile = 32 * P, NT = 64 * P;
     auto& planes = lds.planes;      // Q, dO
     auto& exchange = lds.exchange;
     auto& stats = lds.stats;        // lse (base 2), d
     const int kv = index % a.n_kv;
     Work w;
-    if (!find_work<true, true>(a, kRowsPerWG, 0, index / a.n_kv, &w)) return;
+    if (!find_work<true, true>(a, kTile, 0, index / a.n_kv, &w)) return;
     const Span sp = w.sp;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, c = lane & 31;
-    const int pair = wave & 3, second = wave >> 2;
+    const int pair = wave % P, second = wave / P;
     const int dim = a.head_dim, group = a.group;
     const bool vec = a.vec;
-    const int key0 = w.tile * kRowsPerWG + pair * kRowsPerWave, key = key0 + c;
+    const int key0 = w.tile * kTile + pair * kRowsPerWave, key = key0 + c;
     const bool live = key < (int)sp.kl;
     const int shift = (int)sp.kl - (int)sp.ql, ql = sp.ql;
     const size_t row = sp.k0 + (live ? key : (int)sp.kl - 1);
     const float* k_row = k + row * a.k_rs + (size_t)kv * a.k_hs;
     const float* v_row = v + row * a.v_rs + (size_t)kv * a.v_hs;
     // The tiles of rows that see a key of the work-group, over the group's heads, and this part of them.
-    const int first = max(0, (int)w.tile * kRowsPerWG - shift) / RT, tiles = max(0, (ql + RT - 1) / RT - first);
+    const int first = max(0, (int)w.tile * kTile - shift) / RT, tiles = max(0, (ql + RT - 1) / RT - first);
     const int64_t total = (int64_t)tiles * group;
     const int it0 = (int)(total * part / parts), it1 = (int)(total * (part + 1) / parts);
 
@@ -582,8 +668,8 @@ __device__ __forceinline__ void dkv_tile(BackwardLds<DP>& lds, const PackedAttn&
     load_operand<DP, VEC>(own, second ? v_row : k_row, h, dim);
     floatx16 acc[NB];  // dV^T, dK^T
     clear(acc);
-    // The first four waves stage Q and lse, the others dO and d.
-    Stage<RT, DP, VEC> rows;
+    // The first waves stage Q and lse, the others dO and d.
+    Stage<RT, DP, VEC, NT> rows;
     float stat = 0.f;
     const float* const rows_base = second ? dout + (size_t)sp.q0 * a.o_rs : q + (size_t)sp.q0 * a.q_rs;
     const float* const stat_base = second ? delta : lse;
@@ -591,8 +677,8 @@ __device__ __forceinline__ void dkv_tile(BackwardLds<DP>& lds, const PackedAttn&
     auto load = [&](int it) {
         const int head = kv * group + it / tiles, i0 = (first + it % tiles) * RT;
         rows.load(rows_base + (size_t)head * dim, rows_rs, i0, ql, dim);
-        const int i = i0 + (threadIdx.x & 255);
-        if ((threadIdx.x & 255) < RT) stat = i < ql ? stat_base[(size_t)head * a.q_rows + sp.q0 + i] * (second ? 1.0f : kLog2e) : 0.f;
+        const int i = i0 + (threadIdx.x & (NT - 1));
+        if ((threadIdx.x & (NT - 1)) < RT) stat = i < ql ? stat_base[(size_t)head * a.q_rows + sp.q0 + i] * (second ? 1.0f : kLog2e) : 0.f;
     };
     const float factor = a.scale * kLog2e;
     if (it0 < it1) load(it0);
@@ -600,7 +686,7 @@ __device__ __forceinline__ void dkv_tile(BackwardLds<DP>& lds, const PackedAttn&
         const int i0 = (first + it % tiles) * RT;
         lds_barrier();
         rows.store(planes[second]);
-        if ((threadIdx.x & 255) < RT) stats[second][threadIdx.x & 255] = stat;
+        if ((threadIdx.x & (NT - 1)) < RT) stats[second][threadIdx.x & (NT - 1)] = stat;
         if (it + 1 < it1) load(it + 1);
         lds_barrier();
         floatx16 s[RT / 32];
@@ -658,7 +744,7 @@ __device__ __forceinline__ void dkv_tile(BackwardLds<DP>& lds, const PackedAttn&
     int width = dim;
     if (parts > 1) {
         const size_t tile = (size_t)part * tiles_all + (size_t)w.tile0 * a.n_kv + kv;
-        dst = sums + ((tile * 2 + 1 - second) * kRowsPerWG + key - w.tile * kRowsPerWG) * DP;
+        dst = sums + ((tile * 2 + 1 - second) * kTile + key - w.tile * kTile) * DP;
         dst_vec = true;
         width = DP;
     }
@@ -676,16 +762,18 @@ __device__ __forceinline__ void dkv_tile(BackwardLds<DP>& lds, const PackedAttn&
 
 // The backward pass in one launch: the tiles of dk and dv first (they take longest), then those of dq,
 // which need nothing of them.
-template <int DP, bool VEC>
-__global__ __launch_bounds__(512, DP == 32 ? 4 : 2) void attn_split_backward_kernel(
+template <int DP, bool VEC, int P>
+__global__ __launch_bounds__(128 * P, DP == 32 ? 3 : 2) void attn_split_backward_kernel(
     PackedAttn a, uint32_t key_groups, int parts, float* __restrict__ dq, float* __restrict__ dk, float* __restrict__ dv,
     const float* __restrict__ delta, const float* __restrict__ dout, const float* __restrict__ lse, const float* __restrict__ q,
     const float* __restrict__ k, const float* __restrict__ v, float* __restrict__ sums) {
-    __shared__ BackwardLds<DP> lds;
+    __shared__ BackwardLds<DP, P> lds;
     if (blockIdx.x < key_groups * parts)
-        dkv_tile<DP, VEC>(lds, a, blockIdx.x % key_groups, key_groups, blockIdx.x / key_groups, parts, dk, dv, delta, dout, lse, q, k, v, sums);
+        dkv_tile<DP, VEC, P>(lds, a, blockIdx.x % key_groups, key_groups, blockIdx.x / key_groups, parts, dk, dv, delta, dout, lse, q, k, v, sums);
+    else if constexpr (DP <= 64)
+        dq_tile_alone<DP, VEC, P>(lds, a, blockIdx.x - key_groups * parts, dq, delta, dout, lse, q, k, v);
     else
-        dq_tile<DP, VEC>(lds, a, blockIdx.x - key_groups * parts, dq, delta, dout, lse, q, k, v);
+        dq_tile<DP, VEC, P>(lds, a, blockIdx.x - key_groups * parts, dq, delta, dout, lse, q, k, v);
 }
 
 // d_i = do_i . o_i of every row and head: LPR lanes each.
@@ -710,23 +798,24 @@ __global__ __launch_bounds__(256) void attn_split_delta_kernel(PackedAttn a, flo
 }
 
 // dk and dv of a tile of keys: its parts added in order.
-template <int DP>
+template <int DP, int P>
 __global__ __launch_bounds__(256) void attn_split_dkv_join_kernel(PackedAttn a, float* __restrict__ dk, float* __restrict__ dv,
                                                                   const float* __restrict__ part, int parts) {
+    constexpr int kTile = 32 * P;
     const int kv = blockIdx.x % a.n_kv;
     Work w;
-    if (!find_work<true, true>(a, kRowsPerWG, 0, blockIdx.x / a.n_kv, &w)) return;
-    const int keys = min((int)w.sp.kl - (int)w.tile * kRowsPerWG, kRowsPerWG), dim = a.head_dim;
-    const size_t stride = (size_t)gridDim.x * 2 * kRowsPerWG * DP;
-    const float* p = part + ((size_t)w.tile0 * a.n_kv + kv) * 2 * kRowsPerWG * DP;
-    constexpr int N = 2 * kRowsPerWG * (DP / 4);
+    if (!find_work<true, true>(a, kTile, 0, blockIdx.x / a.n_kv, &w)) return;
+    const int keys = min((int)w.sp.kl - (int)w.tile * kTile, kTile), dim = a.head_dim;
+    const size_t stride = (size_t)gridDim.x * 2 * kTile * DP;
+    const float* p = part + ((size_t)w.tile0 * a.n_kv + kv) * 2 * kTile * DP;
+    constexpr int N = 2 * kTile * (DP / 4);
     for (int e = blockIdx.y * 256 + threadIdx.x; e < N; e += 256 * gridDim.y) {
         const int which = e / (N / 2), key = e % (N / 2) / (DP / 4), d = 4 * (e % (DP / 4));
         if (key >= keys || d >= dim) continue;
         floatx4 x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
         for (int z = 0; z < parts; ++z) x += *reinterpret_cast<const floatx4*>(p + z * stride + 4 * (size_t)e);
-        const size_t row = w.sp.k0 + (size_t)w.tile * kRowsPerWG + key;
+        const size_t row = w.sp.k0 + (size_t)w.tile * kTile + key;
         store4(which ? dv + row * a.v_rs + (size_t)kv * a.v_hs : dk + row * a.k_rs + (size_t)kv * a.k_hs, d, dim, a.vec, x);
     }
 }
@@ -751,9 +840,19 @@ int attn_split_forward(const PackedAttn& a, uint32_t items, uint32_t budget, flo
     return FMLH_OK;
 }
 
+// Pairs of waves per work-group of the backward pass.  At head_dim up to 64 a work-group of two holds half a
+// CU, and two of them are seldom in the same step: 64 x 128 rows, 12 heads of 64, take 116 us with two
+// pairs, 151 with four; 32 x 512 375 and 408.  Long sequences gain by staging a tile for more keys: 4 x 3584 rows,
+// 8 heads, 1040 and 999, 8 x 4096, 16 heads, 5.78 ms and 5.35.
+int attn_split_pairs(const PackedAttn& a) {
+    return a.head_dim > 64 ? PBIG : a.head_dim <= 32 ? 2 : a.k_rows / a.n_seq >= kLongKeys ? 4 : 2;
+}
+int attn_split_dq_rows(const PackedAttn& a) { return (a.head_dim <= 64 ? 64 : 32) * attn_split_pairs(a); }
+int attn_split_back_rows(const PackedAttn& a) { return 32 * attn_split_pairs(a); }
+
 size_t attn_split_part_floats(const PackedAttn& a, uint32_t tiles) {
     const size_t dp = a.head_dim <= 32 ? 32 : a.head_dim <= 64 ? 64 : a.head_dim <= 96 ? 96 : 128;
-    return (size_t)tiles * a.n_kv * 2 * kRowsPerWG * dp;
+    return (size_t)tiles * a.n_kv * 2 * attn_split_back_rows(a) * dp;
 }
 
 int attn_split_backward(const PackedAttn& a, uint32_t row_tiles, uint32_t key_tiles, int parts, float* dq, float* dk, float* dv,
@@ -767,18 +866,28 @@ int attn_split_backward(const PackedAttn& a, uint32_t row_tiles, uint32_t key_ti
     }
     const uint32_t key_groups = key_tiles * a.n_kv;
     const dim3 grid(key_groups * parts + row_tiles * a.n_kv);
-#define FMLH_LAUNCH(DP)                                                                                                               \
-    hipLaunchKernelGGL((a.vec ? attn_split_backward_kernel<DP, true> : attn_split_backward_kernel<DP, false>), grid, dim3(512), 0, s, a, \
-                       key_groups, parts, dq, dk, dv, delta, dout, lse, q, k, v, sums)
-    FMLH_BY_DIM(FMLH_LAUNCH);
-#undef FMLH_LAUNCH
-    FMLH_LAUNCHED("attn_split_backward_kernel");
-    if (parts > 1) {
-#define FMLH_LAUNCH(DP) hipLaunchKernelGGL(attn_split_dkv_join_kernel<DP>, dim3(key_groups, 8), dim3(256), 0, s, a, dk, dv, sums, parts)
-        FMLH_BY_DIM(FMLH_LAUNCH);
-#undef FMLH_LAUNCH
-        FMLH_LAUNCHED("attn_split_dkv_join_kernel");
+#define FMLH_LAUNCH_P(DP, P)                                                                                                            \
+    do {                                                                                                                                \
+        hipLaunchKernelGGL((a.vec ? attn_split_backward_kernel<DP, true, P> : attn_split_backward_kernel<DP, false, P>), grid,          \
+                           dim3(128 * P), 0, s, a, key_groups, parts, dq, dk, dv, delta, dout, lse, q, k, v, sums);                      \
+        FMLH_LAUNCHED("attn_split_backward_kernel");                                                                                    \
+        if (parts > 1) {                                                                                                                \
+            hipLaunchKernelGGL((attn_split_dkv_join_kernel<DP, P>), dim3(key_groups, 8), dim3(256), 0, s, a, dk, dv, sums, parts);       \
+            FMLH_LAUNCHED("attn_split_dkv_join_kernel");                                                                                \
+        }                                                                                                                               \
+    } while (0)
+    const bool two = attn_split_pairs(a) == 2;
+    if (a.head_dim <= 32) {
+        FMLH_LAUNCH_P(32, 2);
+    } else if (a.head_dim <= 64) {
+        if (two) FMLH_LAUNCH_P(64, 2);
+        else FMLH_LAUNCH_P(64, 4);
+    } else if (a.head_dim <= 96) {
+        FMLH_LAUNCH_P(96, PBIG);
+    } else {
+        FMLH_LAUNCH_P(128, PBIG);
     }
+#undef FMLH_LAUNCH_P
     return FMLH_OK;
 }
 
