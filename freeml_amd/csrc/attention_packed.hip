@@ -315,8 +315,15 @@ ForwardPlan plan_forward(const PackedAttn& a) {
     p.per = per_seq > 8 ? kRowsPerWG : per_seq > 4 ? 8 : per_seq > 2 ? 4 : per_seq > 1 ? 2 : 1;
     p.tiles = row_tiles(a, p.per);
     const uint64_t about = std::max<uint64_t>(a.n_seq, (rows + p.per - 1) / p.per) * a.n_kv;
-    const uint64_t want = p.per <= 8 ? 1024 : (getenv("W") ? atoi(getenv("W")) : 512);  // work-groups that keep the device busy
-    p.budget = (getenv("R") ? atoi(getenv("R")) : 2) * about <= 2 * want && keys_per_sequence(a) >= kCutKeys ? (uint32_t)(want / a.n_kv) : 0;
+    // Work-groups to aim at (one that finds no range left costs its start).  Few rows: what keeps the memory busy.
+    // Tiles of rows: two per CU are at work at once up to head_dim 64, and 512 end together (31 queries over 8 x 2000 ..
+    // 32000 keys, 8 heads of 64: 95 us, with 768 121, with 1024 105).  Whole prompts leave the ranges behind a tile's
+    // last row empty (4096 rows, 8 heads of 64: 188 with 512, 154 with 768; 1500 rows, 8 heads of 128: 104, 87
+    // with 768 or 1024).  From 256 tiles on cutting them costs more than it levels: 4 x 1024 rows, 12 heads of 64, 87 us
+    // whole, 113 cut.
+    const bool prompts = 2 * (uint64_t)a.q_rows > keys_per_sequence(a) * a.n_seq;
+    const uint64_t want = p.per <= 8 ? 1024 : prompts ? 768 : 512;
+    p.budget = about <= (p.per <= 8 ? 512 : 256) && keys_per_sequence(a) >= kCutKeys ? (uint32_t)(want / a.n_kv) : 0;
     return p;
 }
 
