@@ -165,6 +165,28 @@ def test_8_bit_states(gap, seed):
 
 
 @pytest.mark.gpu
+def test_quotients_and_roots_of_every_mantissa():
+    """The quick forms of the update's divisions and root against the single update's, for every mantissa of v of an
+    even and an odd exponent: with beta 1 and powers 0 the states stay, and p takes lr m / (sqrt(v) + eps)."""
+    n = 1 << 24
+    v = (np.arange(n, dtype=np.uint32) + (np.uint32(120) << np.uint32(23))).view(F)
+    m = np.random.default_rng(0).standard_normal(n).astype(F)
+    zero = np.zeros(n, F)
+    d = [[fh.DeviceArray.from_host(x) for x in (zero, zero, m, v)] for _ in range(2)]
+    fh.adamw_update_multi(fh.adamw_tensors([(*(x.ptr for x in d[0]), n)]), 32, LR, 1.0, 1.0, 0.0, 0.0, 2.0**-48, 0.0)
+    fh.adamw_update(*(x.ptr for x in d[1]), n, LR, 1.0, 1.0, 0.0, 0.0, 2.0**-48, 0.0)
+    for a, b in zip(*d):
+        np.testing.assert_array_equal(a.numpy(), b.numpy())
+    # Divisors that are not 1: every mantissa of m and v against an arbitrary 1 - beta^t.
+    m2 = np.where(np.arange(n) % 2 == 0, v, -v).astype(F)
+    d = [[fh.DeviceArray.from_host(x) for x in (zero, zero, m2, v)] for _ in range(2)]
+    for p1, p2 in ((0.9, 0.999), (0.1234, 0.77)):
+        fh.adamw_update_multi(fh.adamw_tensors([(*(x.ptr for x in d[0]), n)]), 32, LR, 1.0, 1.0, p1, p2, EPS, 0.0)
+        fh.adamw_update(*(x.ptr for x in d[1]), n, LR, 1.0, 1.0, p1, p2, EPS, 0.0)
+        np.testing.assert_array_equal(d[0][0].numpy(), d[1][0].numpy())
+
+
+@pytest.mark.gpu
 def test_8_bit_update_against_64_bits():
     """One step from states of zero: m and v are exact before they are rounded, so p is off by the
     formula's own roundings, six of them at most half a step each, relative to the update, and one of p."""

@@ -258,6 +258,21 @@ def test_queries_over_longer_keys(layout, qlens, klens, heads, kv_heads, dim):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("lens,heads,kv_heads,dim", [([1700], 2, 1, 64), ([1600, 1550], 1, 1, 33), ([2100], 1, 1, 24), ([900, 1300], 2, 2, 128)])
+def test_long_sequences(lens, heads, kv_heads, dim):
+    """From 1536 keys on four pairs of waves share a tile of the backward pass; few tiles of long keys are cut."""
+    check(Case(lens, lens, heads, kv_heads, dim, extra=(1, 0), seed=dim))
+
+
+@pytest.mark.gpu
+def test_more_work_than_runs_at_once():
+    """Up to 64 sequences in the order of their work: every tile once, whatever the lengths."""
+    r = np.random.default_rng(5)
+    lens = r.integers(0, 400, 60).tolist()
+    check(Case(lens, lens, 6, 6, 16, seed=11))
+
+
+@pytest.mark.gpu
 def test_many_sequences():
     r = np.random.default_rng(4)
     lens = r.integers(0, 12, 300).tolist()
@@ -269,6 +284,27 @@ def test_many_sequences():
 def test_sizes_of_values(std):
     """Scores near zero (an even softmax) and in the thousands (one key takes all)."""
     check(Case([90, 40], [90, 40], 4, 2, 64, seed=5, std=std, scale=0.125 if std < 1e3 else 1e-6))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [32, 64, 128])
+@pytest.mark.parametrize("v,g", [(1e30, 1.0), (1e-30, 1e30), (1.0, 1e-34), (1e-34, 1.0), (1e34, 1e-34), (1e-20, 1e-12)])
+def test_values_and_gradients_at_the_ends_of_the_range(v, g, dim):
+    """Operands whose parts or sums leave the range of the bf16 products, at either end, lose nothing."""
+    c = Case([70, 33], [70, 33], 4, 2, dim, seed=13)
+    c.v = [(x * np.float32(v)).astype(np.float32) for x in c.v]
+    c.g = [(x * np.float32(g)).astype(np.float32) for x in c.g]
+    check(c)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("klens", [[3000], [900, 2000]])
+def test_cut_keys_at_the_ends_of_the_range(klens):
+    """The same where the keys are cut into ranges, on tiles of rows and on few rows."""
+    for n in (40, 1):
+        c = Case([n] * len(klens), klens, 4, 2, 64, "cache", seed=14)
+        c.v = [x * np.float32(1e30) for x in c.v]
+        check(c, backward=False)
 
 
 @pytest.mark.gpu
