@@ -9,6 +9,9 @@
 // probability of m's (of v's, the square's) distance from below, so that m and v are kept on average.
 // The 16 random bits of either come from a hash of the seed, the tensor's number and the element's.  A
 // positive r keeps at least the smallest code: rounded to zero, its update would be divided by eps alone.
+//
+// The bytes bound it: 10.7M elements with 32-bit states 63 us (301 MB, 4.75 TB/s), 124M with 8-bit ones 430 us (2.0 GB,
+// 4.6 TB/s; a copy reaches 5.05).  With compiler divisions and roots, and one block per wave, 92 and 671.
 #include "fmlh_internal.h"
 
 #include <algorithm>

@@ -16,6 +16,15 @@
 //     taking the rows in this order as the 8 k of a half makes probabilities and their gradients
 //     the next product's operand without leaving the registers.
 //   * A tile's rows are requested into registers while the tile before them is multiplied.
+//
+// What bounds them: at 8 x 4096 rows, 16 heads of 64, the forward pass runs at 180 TFLOP/s of the 234 that a
+// sixth of a large bf16 product is (matrix cores 54% and vector units 60% of the clocks, which the power
+// limit holds at 1.9 GHz); the fp32 matrix cores' 151 would leave 97.  The backward pass forms seven products
+// for the five that have to be (S and dP twice, so that no sum crosses work-groups): 131 TFLOP/s of the five,
+// 184 of the seven.  Short sequences are bound by the chain of one wave: offsets, loads, S, softmax, P V, 10 us for one tile.
+// Measured and not kept: the next tile's S among this one's softmax, in program order or by scheduling
+// groups (D 64 -2 .. +4%, D 128 +9%, shorter sequences 5 - 10% slower); pairs of waves for dq up to
+// head_dim 64 (8 x 4096 rows, 16 heads: 5.76 ms for the pass, 5.22); keys cut into ranges from 256 tiles on.
 #include "attention_packed_device.h"
 
 namespace fmlh {
@@ -242,9 +251,8 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attn_split_kernel(Packe
     const int qi = (live ? rho : rows - 1) / group, head = kv * group + (live ? rho : rows - 1) % group;
     const int limit = min(qi + shift, k_end - 1);  // last key of the range that this row sees
     // Over the wave's rows (uniform): the first row's limit, and the last one's.
-    const int first_limit = min(rho0, rows - 1) / group + shift, last_limit = min(rho0 + kRowsPerWave, rows) - 1 < rho0
-                                                                                  ? -1
-                                                                                  : (min(rho0 + kRowsPerWave, rows) - 1) / group + shift;
+    const int first_limit = min(rho0, rows - 1) / group + shift;
+    const int last_limit = rho0 < rows ? (min(rho0 + kRowsPerWave, rows) - 1) / group + shift : -1;
     const float* kb = k + (size_t)sp.k0 * a.k_rs + (size_t)kv * a.k_hs;
     const float* vb = v + (size_t)sp.k0 * a.v_rs + (size_t)kv * a.v_hs;
     const float* q_row = q + (size_t)(sp.q0 + qi) * a.q_rs + (size_t)head * dim;
@@ -427,9 +435,6 @@ __device__ __noinline__ void redo_dkv(Redone<DP>& result, const PackedAttn& a, c
 }
 
 // Keys of a sequence from which on a work-group of the backward pass has four pairs of waves.
-#ifndef PBIG
-#define PBIG 4
-#endif
 constexpr uint32_t kLongKeys = 1536;
 
 // Tiles of the backward pass: 64 rows or keys in LDS at head_dim 33 .. 64, else 32 (LDS at 128 would hold no more;
@@ -631,7 +636,7 @@ __device__ __forceinline__ void dq_tile_alone(BackwardLds<DP, P>& lds, const Pac
 
 // dk and dv: a work-group per tile of keys of one (sequence, key head), a key per lane column; the rows of
 // the group's heads stream through LDS.  Two waves share 32 keys (keeping K and V parts and both sums
-// in one wave's registers spilled at head_dim 128: 4.9 ms where this takes @DKV128@):
+// in one wave's registers spilled at head_dim 128: 4.9 ms for two sequences of 3000 .. 4096, 16 heads on 2; 1.8 so):
 //   the first   S = Q K^T, p, dV^T += dO^T P     holds K and dV,
 //   the second  dP = dO V^T, dS, dK^T += Q^T dS  holds V and dK and takes p from the first.
 // Where there are few such tiles, their rows are cut into parts (whole tiles of rows, of all heads in
@@ -842,10 +847,12 @@ int attn_split_forward(const PackedAttn& a, uint32_t items, uint32_t budget, flo
 
 // Pairs of waves per work-group of the backward pass.  At head_dim up to 64 a work-group of two holds half a
 // CU, and two of them are seldom in the same step: 64 x 128 rows, 12 heads of 64, take 116 us with two
-// pairs, 151 with four; 32 x 512 375 and 408.  Long sequences gain by staging a tile for more keys: 4 x 3584 rows,
-// 8 heads, 1040 and 999, 8 x 4096, 16 heads, 5.78 ms and 5.35.
+// pairs, 151 with four; 32 x 512 375 and 408; 24 x 100 .. 2048, 12 heads on 4, 583 and 640.  Long sequences gain by staging
+// a tile for more keys: 8 x 2048, 12 heads, 1100 and 1040, 8 x 4096, 16 heads, 5.75 ms and 5.22.  At head_dim 32 two
+// fit three times (8 x 4096, 16 heads, 3.05 ms, four pairs 3.15); beyond 64 four pairs, whose staging takes half the registers
+// (4 x 4096, 16 heads of 128, 5.6 ms, with two 10.4).
 int attn_split_pairs(const PackedAttn& a) {
-    return a.head_dim > 64 ? PBIG : a.head_dim <= 32 ? 2 : a.k_rows / a.n_seq >= kLongKeys ? 4 : 2;
+    return a.head_dim > 64 ? 4 : a.head_dim <= 32 ? 2 : a.k_rows / a.n_seq >= kLongKeys ? 4 : 2;
 }
 int attn_split_dq_rows(const PackedAttn& a) { return (a.head_dim <= 64 ? 64 : 32) * attn_split_pairs(a); }
 int attn_split_back_rows(const PackedAttn& a) { return 32 * attn_split_pairs(a); }
@@ -883,9 +890,9 @@ int attn_split_backward(const PackedAttn& a, uint32_t row_tiles, uint32_t key_ti
         if (two) FMLH_LAUNCH_P(64, 2);
         else FMLH_LAUNCH_P(64, 4);
     } else if (a.head_dim <= 96) {
-        FMLH_LAUNCH_P(96, PBIG);
+        FMLH_LAUNCH_P(96, 4);
     } else {
-        FMLH_LAUNCH_P(128, PBIG);
+        FMLH_LAUNCH_P(128, 4);
     }
 #undef FMLH_LAUNCH_P
     return FMLH_OK;

@@ -50,7 +50,8 @@ def reference(off, z, t, ref, beta, smoothing):
     x = beta * (ratio[0::2] - ratio[1::2])
     b_x = beta * (b_lp[0::2] + b_lp[1::2])
     loss = (1 - smoothing) * np.logaddexp(0, -x) + (smoothing * np.logaddexp(0, x) if smoothing else 0.0)
-    f = beta / P * ((1 - smoothing) / (1 + np.exp(x)) - smoothing / (1 + np.exp(-x)))
+    with np.errstate(over="ignore"):
+        f = beta / P * ((1 - smoothing) / (1 + np.exp(x)) - smoothing / (1 + np.exp(-x)))
     grad, b_grad = np.full(z.shape, float(MARK)), np.zeros(z.shape)
     onehot = np.zeros(z.shape)
     onehot[np.nonzero(ok)[0], ids[ok]] = 1.0
