@@ -5,13 +5,16 @@
 
 namespace fmlh {
 
+// Row stride in floats up to which a tile of 64 rows lies inside the 31 bits of a buffer's offsets.
+constexpr size_t kMaxVecStride = size_t(1) << 22;
+
 struct PackedAttn {
     uint32_t n_seq, q_rows, k_rows;
     int group;     // query heads per key head
     uint32_t n_kv; // key heads
     int head_dim;
     float scale;
-    int vec;       // every row and head 16-byte aligned, head_dim a multiple of 4
+    int vec;       // every row and head 16-byte aligned, head_dim a multiple of 4, row strides up to kMaxVecStride
     const int32_t *q_off, *k_off, *k_len;
     size_t q_rs, k_rs, v_rs, o_rs, k_hs, v_hs;
 };

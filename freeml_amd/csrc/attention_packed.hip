@@ -286,7 +286,8 @@ PackedAttn make_args(const fmlh_packed_attention* s) {
     a.k_hs = s->k_hs;
     a.v_hs = s->v_hs;
     a.vec = s->head_dim % 4 == 0 && ((s->q_rs | s->k_rs | s->v_rs | s->o_rs) & 3) == 0 &&
-            (s->n_kv_head == 1 || ((s->k_hs | s->v_hs) & 3) == 0);
+            (s->n_kv_head == 1 || ((s->k_hs | s->v_hs) & 3) == 0) &&
+            std::max({s->q_rs, s->k_rs, s->v_rs, s->o_rs}) <= kMaxVecStride;
     return a;
 }
 

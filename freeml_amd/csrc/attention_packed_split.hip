@@ -46,27 +46,33 @@ template <int R, int DP, bool VEC, int NT = 256>
 struct Stage {
     static constexpr int U = DP / 8, N = (R * U + NT - 1) / NT;
     floatx4 x[N][2];
-    // Rows first .. of a matrix at base (64-bit, uniform), row stride rs; rows from `rows` on (rows > first) are zeros.
+    // Rows first .. of a matrix at base (64-bit, uniform), row stride rs; rows from `rows` on (rows > first) and
+    // dims from `dim` on are zeros.  VEC: by buffer loads, whose range check gives the zeros, so that no value is
+    // waited for here; offsets stay inside 31 bits (kMaxVecStride).
     __device__ __forceinline__ void load(const float* base, size_t rs, int first, int rows, int dim) {
         const int t = threadIdx.x & (NT - 1);
         const float* tile = base + (size_t)first * rs;
-        if (VEC && R * U % NT == 0 && first + R <= rows && dim == DP) {
+        const int left = min(rows - first, R);
+        if constexpr (VEC) {
+            const int stride = (int)rs * 4, bytes = __builtin_amdgcn_readfirstlane((left - 1) * stride + 4 * dim);
+            const uint64_t start = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)((uint64_t)tile >> 32)) << 32 |
+                                   (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint64_t)tile);
+            const __amdgpu_buffer_rsrc_t buffer = __builtin_amdgcn_make_buffer_rsrc((float*)start, 0, bytes, 0x00020000);
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                const int u = t + NT * i;
-                const floatx4* row = reinterpret_cast<const floatx4*>(tile + (size_t)(u / U) * rs + 8 * (u % U));
-                x[i][0] = row[0];
-                x[i][1] = row[1];
+                const int u = t + NT * i, d = 8 * (u % U), at = u / U * stride + 4 * d;
+                x[i][0] = __builtin_bit_cast(floatx4, __builtin_amdgcn_raw_buffer_load_b128(buffer, d < dim ? at : bytes, 0, 0));
+                x[i][1] = __builtin_bit_cast(floatx4, __builtin_amdgcn_raw_buffer_load_b128(buffer, d + 4 < dim ? at + 16 : bytes, 0, 0));
             }
-            return;
-        }
+        } else {
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int u = min(t + NT * i, R * U - 1), r = u / U, d = 8 * (u % U);
-            const bool on = first + r < rows;
-            const float* row = tile + (size_t)(on ? r : 0) * rs;
-            x[i][0] = load4_padded<VEC>(row, d, dim, on);
-            x[i][1] = load4_padded<VEC>(row, d + 4, dim, on);
+            for (int i = 0; i < N; ++i) {
+                const int u = min(t + NT * i, R * U - 1), r = u / U, d = 8 * (u % U);
+                const bool on = r < left;
+                const float* row = tile + (size_t)(on ? r : 0) * rs;
+                x[i][0] = load4_padded<false>(row, d, dim, on);
+                x[i][1] = load4_padded<false>(row, d + 4, dim, on);
+            }
         }
     }
     __device__ __forceinline__ void store(uintx4* planes) const {
@@ -234,7 +240,7 @@ template <int DP, bool VEC>
 __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attn_split_kernel(PackedAttn a, float* __restrict__ out, float* __restrict__ lse,
                                                             const float* __restrict__ q, const float* __restrict__ k,
                                                             const float* __restrict__ v, float* __restrict__ ws, uint32_t budget) {
-    constexpr int KT = DP <= 64 ? 64 : 32, U = DP / 8, NB = DP / 32;
+    constexpr int KT = 64, U = DP / 8, NB = DP / 32;
     __shared__ uintx4 kp[3 * KT * U];
     __shared__ uintx4 vp[3 * KT * U];
     const int kv = blockIdx.x % a.n_kv;
