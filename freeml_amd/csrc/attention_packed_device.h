@@ -84,16 +84,19 @@ __device__ __forceinline__ bool find_work(const PackedAttn& a, uint32_t per_tile
     Span p{};
     w->per = 0x40000000;
     if (budget) {
+        // Keys of all tiles, in integers, so that every work-group and launch has the same: sums of 20 bits and of
+        // the rest (cut launches have at most about 1000 tiles, so 2^41 keys of a sequence's).
         uint64_t keys = 0;
         for (uint32_t base = 0; base < a.n_seq; base += 64) {
             p = Span{};
             if (base + lane < a.n_seq) p = load_span(a, base + lane);
-            keys += (uint64_t)tiles_of(p) * p.kl;
+            const uint64_t x = (uint64_t)tiles_of(p) * p.kl;
+            keys += wave_sum_int((int)(x & 0xfffff)) + ((uint64_t)wave_sum_int((int)(x >> 20)) << 20);
         }
-#pragma unroll
-        for (int d = 32; d >= 1; d >>= 1) keys += __shfl_xor((unsigned long long)keys, d);
-        const uint64_t least = per_tile <= 8 ? 128 : 256, per = ((keys + budget - 1) / budget + least - 1) / least * least;
-        w->per = (int)min(per, (uint64_t)0x40000000);
+        // An equal share, rounded up to whole `least`: 1 + 2^-18 covers the roundings of this quotient.
+        const int least = per_tile <= 8 ? 128 : 256;
+        const float share = __fmul_rn(__fmul_rn((float)keys, 1.0f + 0x1p-18f), __builtin_amdgcn_rcpf((float)(budget * least)));
+        w->per = max(1, (int)ceilf(fminf(share, 0x1p30f / least))) * least;
     }
     if (!budget && a.n_seq <= 64 && gridDim.x > kAtOnce) {
         if (lane < a.n_seq) p = load_span(a, lane);

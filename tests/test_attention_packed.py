@@ -273,6 +273,19 @@ def test_more_work_than_runs_at_once():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("qlens", [[1, 1, 1], [3, 2, 2], [200, 70, 300]])
+def test_caches_without_a_key(qlens):
+    """Room for many keys, none of them written: every row is there and empty."""
+    c = Case(qlens, [900, 800, 700], 4, 2, 64, "cache").build()
+    c.klens = [0, 0, 0]
+    c.d_off[2].upload(np.zeros(3, np.int32))
+    c.forward()
+    out, lse = c.d_out.numpy(), c.d_lse.numpy()
+    assert all(np.all(x == 0.0) for x in c.read_rows(out)) and np.all(lse == -np.inf)
+    c.untouched(out, "out")
+
+
+@pytest.mark.gpu
 def test_many_sequences():
     r = np.random.default_rng(4)
     lens = r.integers(0, 12, 300).tolist()
