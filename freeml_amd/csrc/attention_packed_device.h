@@ -67,7 +67,7 @@ constexpr uint32_t kAtOnce = 512;  // work-groups of attention kernels on the de
 // and every one of them its keys' ranges.  `budget` ranges are spread over all tiles: one has the
 // keys of all tiles / budget, so that long sequences are cut and short ones are not (budget 0: none
 // is), and at least 128, or 256 for tiles of more rows: those start and end in the time of 256 keys
-// (48 queries of 16 heads of 80 on 4 over 500 .. 4000 keys: 52 us with 128, 46 with 256).
+// (48 queries of 16 heads of 80 on 4 over 500 .. 4000 keys: 44 us with 128, 40 with 256).
 // Every wave scans the offsets, 64 sequences at a time.  False behind the last sequence: grids hold
 // sum / per_tile + n_seq tiles and budget items more, never fewer than there are.
 // Up to 64 sequences whose keys are not cut come in the order of their work, most first over all of

@@ -15,9 +15,11 @@
 //   * A lane's accumulator registers 8 t .. 8 t + 7 are rows 16 t + 4 h + {0..3, 8..11} of its column:
 //     taking the rows in this order as the 8 k of a half makes probabilities and their gradients
 //     the next product's operand without leaving the registers.
-//   * A tile's rows are requested into registers while the tile before them is multiplied.
+//   * A tile's rows are requested into registers while the tile before them is multiplied, by buffer loads whose
+//     range check gives the zeros behind a sequence or a head (with the zeros chosen after an ordinary load every
+//     such tile waited for its values: 48 queries over 500 .. 4000 keys, 16 heads of 80 on 4, 41.4 us, 37.5 so).
 //
-// What bounds them: at 8 x 4096 rows, 16 heads of 64, the forward pass runs at 180 TFLOP/s of the 234 that a
+// What bounds them: at 8 x 4096 rows, 16 heads of 64, the forward pass runs at 178 TFLOP/s of the 234 that a
 // sixth of a large bf16 product is (matrix cores 54% and vector units 60% of the clocks, which the power
 // limit holds at 1.9 GHz); the fp32 matrix cores' 151 would leave 97.  The backward pass forms seven products
 // for the five that have to be (S and dP twice, so that no sum crosses work-groups): 131 TFLOP/s of the five,
