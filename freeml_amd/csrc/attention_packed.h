@@ -21,8 +21,8 @@ struct PackedAttn {
 
 // The kernels on the bf16 matrix cores (attention_packed_split.hip).  Grids hold `items` / `tiles` per
 // key head; ws, delta and sums are workspace.
-int attn_split_forward(const PackedAttn& a, uint32_t items, uint32_t budget, float* out, float* lse, const float* q, const float* k,
-                       const float* v, float* ws, hipStream_t s);
+int attn_split_forward(const PackedAttn& a, int per, uint32_t items, uint32_t budget, float* out, float* lse, const float* q,
+                       const float* k, const float* v, float* ws, hipStream_t s);
 // Rows, or keys, of a tile of the backward pass.
 int attn_split_dq_rows(const PackedAttn& a);
 int attn_split_back_rows(const PackedAttn& a);

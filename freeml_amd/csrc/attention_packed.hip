@@ -184,55 +184,58 @@ __global__ __launch_bounds__(256) void attn_packed_few_kernel(PackedAttn a, floa
     }
 }
 
-// Joins the ranges of the rows whose keys were cut into more than one: a wave per row, four rows of a
-// tile per work-group; the ranges' outputs are added in range order.
+// Joins the ranges of the rows whose keys were cut into more than one: a wave per row, the ranges'
+// outputs added in range order.  A work-group takes four rows of a tile at a time; about 2048 of them are
+// launched, since each has to find its tile first.
 template <int TILE>
 __global__ __launch_bounds__(256) void attn_packed_join_kernel(PackedAttn a, float* __restrict__ out, float* __restrict__ lse,
                                                                float* __restrict__ ws, uint32_t budget, uint32_t items) {
     Work w;
     if (!find_work<false, true>(a, TILE, budget, blockIdx.x, &w)) return;
     const RowTile tl = row_tile(a, w, TILE);
-    const int lane = threadIdx.x & 63, t = blockIdx.z * 4 + (threadIdx.x >> 6), rho = tl.rho0 + t;
-    if (tl.ranges == 1 || rho > tl.last) return;
-    const int dim = a.head_dim, group = a.group, kv = blockIdx.y;
-    const size_t head = (size_t)kv * group + rho % group, row = w.sp.q0 + rho / group;
+    if (tl.ranges == 1) return;
+    const int lane = threadIdx.x & 63, dim = a.head_dim, group = a.group, kv = blockIdx.y;
     const Partials part = partials(ws, gridDim.y, kv, items, w.item0, TILE, dim);
-    float top = -INFINITY;
-    for (int z = lane; z < tl.ranges; z += 64) top = fmaxf(top, part.ml[2 * (z * TILE + t)]);
-    top = wave_max(top);
-    const float base = top == -INFINITY ? 0.f : top;
-    float sum = 0.f, x[2] = {0.f, 0.f};
-    for (int z0 = 0; z0 < tl.ranges; z0 += 64) {
-        const int z = z0 + lane;
-        float corr = 0.f;
-        if (z < tl.ranges) {
-            corr = exp2f(part.ml[2 * (z * TILE + t)] - base);
-            sum += part.ml[2 * (z * TILE + t) + 1] * corr;
-        }
-        const int n = min(64, tl.ranges - z0);
-        for (int i0 = 0; i0 < n; i0 += 8) {
-            float y[8][2];
+    for (int t = blockIdx.z * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); tl.rho0 + t <= tl.last; t += 4 * gridDim.z) {
+        const int rho = tl.rho0 + t;
+        const size_t head = (size_t)kv * group + rho % group, row = w.sp.q0 + rho / group;
+        float top = -INFINITY;
+        for (int z = lane; z < tl.ranges; z += 64) top = fmaxf(top, part.ml[2 * (z * TILE + t)]);
+        top = wave_max(top);
+        const float base = top == -INFINITY ? 0.f : top;
+        float sum = 0.f, x[2] = {0.f, 0.f};
+        for (int z0 = 0; z0 < tl.ranges; z0 += 64) {
+            const int z = z0 + lane;
+            float corr = 0.f;
+            if (z < tl.ranges) {
+                corr = exp2f(part.ml[2 * (z * TILE + t)] - base);
+                sum += part.ml[2 * (z * TILE + t) + 1] * corr;
+            }
+            const int n = min(64, tl.ranges - z0);
+            for (int i0 = 0; i0 < n; i0 += 8) {
+                float y[8][2];
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
+                for (int i = 0; i < 8; ++i)
 #pragma unroll
-                for (int e = 0; e < 2; ++e)
-                    y[i][e] = lane + 64 * e < dim ? part.o[((size_t)min(z0 + i0 + i, tl.ranges - 1) * TILE + t) * padded_dim(dim) + lane + 64 * e] : 0.f;
+                    for (int e = 0; e < 2; ++e)
+                        y[i][e] = lane + 64 * e < dim ? part.o[((size_t)min(z0 + i0 + i, tl.ranges - 1) * TILE + t) * padded_dim(dim) + lane + 64 * e] : 0.f;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float c = __shfl(corr, i0 + i);
+                for (int i = 0; i < 8; ++i) {
+                    const float c = __shfl(corr, i0 + i);
 #pragma unroll
-                for (int e = 0; e < 2; ++e)
-                    if (i0 + i < n) x[e] += y[i][e] * c;
+                    for (int e = 0; e < 2; ++e)
+                        if (i0 + i < n) x[e] += y[i][e] * c;
+                }
             }
         }
-    }
-    sum = wave_sum(sum);
-    const float inv = rho / group + tl.shift < 0 ? 0.f : 1.0f / sum;
-    float* dst = out + row * a.o_rs + head * dim;
+        sum = wave_sum(sum);
+        const float inv = rho / group + tl.shift < 0 ? 0.f : 1.0f / sum;
+        float* dst = out + row * a.o_rs + head * dim;
 #pragma unroll
-    for (int e = 0; e < 2; ++e)
-        if (lane + 64 * e < dim) dst[lane + 64 * e] = x[e] * inv;
-    if (lse && lane == 0) lse[head * a.q_rows + row] = (top + log2f(sum)) * kLn2;
+        for (int e = 0; e < 2; ++e)
+            if (lane + 64 * e < dim) dst[lane + 64 * e] = x[e] * inv;
+        if (lse && lane == 0) lse[head * a.q_rows + row] = (top + log2f(sum)) * kLn2;
+    }
 }
 
 // ---- host ------------------------------------------------------------------------------------
@@ -305,7 +308,7 @@ uint64_t keys_per_sequence(const PackedAttn& a) {
 
 // How the forward pass cuts its work, by the sizes alone (lengths are the device's to know).
 struct ForwardPlan {
-    int per;          // rows per tile: kRowsPerWG, or at most 8 for attn_packed_few_kernel
+    int per;          // rows per tile: kRowsPerWG or half of it, or at most 8 for attn_packed_few_kernel
     uint32_t tiles;   // at most, for a key head
     uint32_t budget;  // ranges to cut the tiles' keys into, for a key head; 0: none
 };
@@ -315,17 +318,23 @@ ForwardPlan plan_forward(const PackedAttn& a) {
     const uint64_t rows = (uint64_t)a.q_rows * a.group;  // of a key head
     const uint64_t per_seq = rows / a.n_seq;
     p.per = per_seq > 8 ? kRowsPerWG : per_seq > 4 ? 8 : per_seq > 2 ? 4 : per_seq > 1 ? 2 : 1;
-    p.tiles = row_tiles(a, p.per);
     const uint64_t about = std::max<uint64_t>(a.n_seq, (rows + p.per - 1) / p.per) * a.n_kv;
+    const bool prompts = 2 * (uint64_t)a.q_rows > keys_per_sequence(a) * a.n_seq, enough = keys_per_sequence(a) >= kCutKeys;
     // Work-groups to aim at (one that finds no range left costs its start).  Few rows: what keeps the memory busy.
     // Tiles of rows: two per CU are at work at once up to head_dim 64, and 512 end together (31 queries over 8 x 2000 ..
     // 32000 keys, 8 heads of 64: 95 us, with 768 121, with 1024 105).  Whole prompts leave the ranges behind a tile's
     // last row empty (4096 rows, 8 heads of 64: 188 with 512, 154 with 768; 1500 rows, 8 heads of 128: 104, 87
-    // with 768 or 1024).  From 256 tiles on cutting them costs more than it levels: 4 x 1024 rows, 12 heads of 64, 87 us
-    // whole, 113 cut.
-    const bool prompts = 2 * (uint64_t)a.q_rows > keys_per_sequence(a) * a.n_seq;
+    // with 768 or 1024).
     const uint64_t want = p.per <= 8 ? 1024 : prompts ? 768 : 512;
-    p.budget = about <= (p.per <= 8 ? 512 : 256) && keys_per_sequence(a) >= kCutKeys ? (uint32_t)(want / a.n_kv) : 0;
+    // Tiles up to which cutting pays.  Prompts: 2048 rows, 8 heads of 64 (128 tiles), 66 us cut, 76 whole; 16 heads
+    // 96 and 82; 4 x 1024 rows, 8 heads of 128 (256), 147 and 94.
+    const uint64_t few = p.per <= 8 ? 512 : prompts ? 128 : 256;
+    p.budget = about <= few && enough ? (uint32_t)(want / a.n_kv) : 0;
+    // Half the rows a tile, the keys shared by pairs of waves, where whole tiles leave CUs empty or ending early: 16 x
+    // 20 .. 256 rows, 6 heads (126 tiles), 13.6 us, 17.0 with all rows; 4 x 1024, 12 heads (384), 65 and 82.  Short rows
+    // lose where tiles are many (32 x 256, 6 heads, 384 tiles, 31.6 and 27.8), long ones too (16 x 512, 8 heads, 512, 49 and 44).
+    if (p.per == kRowsPerWG && !p.budget && about <= (enough ? 400 : 256)) p.per = kRowsPerWG / 2;
+    p.tiles = row_tiles(a, p.per);
     return p;
 }
 
@@ -404,11 +413,11 @@ int fmlh_attention_packed(const fmlh_packed_attention* shape, float* out, float*
 #undef FMLH_FEW
         FMLH_LAUNCHED("attn_packed_few_kernel");
     } else {
-        FMLH_TRY(attn_split_forward(a, items, plan.budget, out, lse, q, k, v, ws, stream()));
+        FMLH_TRY(attn_split_forward(a, plan.per, items, plan.budget, out, lse, q, k, v, ws, stream()));
     }
     if (plan.budget) {
 #define FMLH_JOIN(TILE)                                                                                                      \
-    hipLaunchKernelGGL(attn_packed_join_kernel<TILE>, dim3(plan.tiles, a.n_kv, (TILE + 3) / 4), dim3(256), 0, stream(), a, out, \
+    hipLaunchKernelGGL(attn_packed_join_kernel<TILE>, dim3(plan.tiles, a.n_kv, std::clamp<uint32_t>(2048 / (plan.tiles * a.n_kv), 1, (TILE + 3) / 4)), dim3(256), 0, stream(), a, out, \
                        lse, ws, plan.budget, items)
         switch (plan.per) {
             case 1: FMLH_JOIN(1); break;

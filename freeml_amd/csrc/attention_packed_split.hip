@@ -238,20 +238,23 @@ __device__ __noinline__ void redo_rows(Redone<DP>& result, const PackedAttn& a, 
     result.l = l;
 }
 
-template <int DP, bool VEC>
+// PER rows per work-group: four waves of 32, or two pairs (64), whose second waves take the second half of every
+// tile of keys and hand over their maxima, sums and outputs at the end.
+template <int DP, bool VEC, int PER>
 __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attn_split_kernel(PackedAttn a, float* __restrict__ out, float* __restrict__ lse,
                                                             const float* __restrict__ q, const float* __restrict__ k,
                                                             const float* __restrict__ v, float* __restrict__ ws, uint32_t budget) {
-    constexpr int KT = 64, U = DP / 8, NB = DP / 32;
-    __shared__ uintx4 kp[3 * KT * U];
-    __shared__ uintx4 vp[3 * KT * U];
+    constexpr int KT = 64, U = DP / 8, NB = DP / 32, WAVES = PER / kRowsPerWave, KB = KT / 32 * WAVES / 4;
+    __shared__ uintx4 planes[2][3 * KT * U];
+    uintx4 *const kp = planes[0], *const vp = planes[1];
     const int kv = blockIdx.x % a.n_kv;
     Work w;
-    if (!find_work<false, false>(a, kRowsPerWG, budget, blockIdx.x / a.n_kv, &w)) return;
-    const RowTile tl = row_tile(a, w, kRowsPerWG);
+    if (!find_work<false, false>(a, PER, budget, blockIdx.x / a.n_kv, &w)) return;
+    const RowTile tl = row_tile(a, w, PER);
     if (w.range >= tl.ranges) return;
     const Span sp = w.sp;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, c = lane & 31;
+    const int lane = threadIdx.x & 63, h = lane >> 5, c = lane & 31;
+    const int all = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wave = all % WAVES, part0 = all / WAVES * KB * 32;
     const int dim = a.head_dim, group = a.group, rows = tl.rows, shift = tl.shift, k_begin = tl.k_begin, k_end = tl.k_end;
     const bool vec = a.vec;
     const int rho0 = tl.rho0 + wave * kRowsPerWave, rho = rho0 + c;
@@ -316,13 +319,39 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attn_split_kernel(Packe
             vs.load(vb, a.v_rs, t0 + KT, k_end, dim);
         }
         lds_barrier();
-        if (t0 > last_limit) continue;  // no row of the wave sees the tile
-        floatx16 s[KT / 32];
+        if (t0 + part0 > min(last_limit, k_end - 1)) continue;  // no row of the wave sees its keys of the tile
+        floatx16 s[KB];
 #pragma unroll
-        for (int j = 0; j < KT / 32; ++j) s[j] = tile_product<KT, DP>(kp, 32 * j, qp, h, c);
-        softmax(s, KT / 32, t0, factor * kDown2);
+        for (int j = 0; j < KB; ++j) s[j] = tile_product<KT, DP>(kp, part0 + 32 * j, qp, h, c);
+        softmax(s, KB, t0 + part0, factor * kDown2);
 #pragma unroll
-        for (int j = 0; j < KT / 32; ++j) tile_add<KT, DP>(o, vp, 32 * j, s[j], lane);
+        for (int j = 0; j < KB; ++j) tile_add<KT, DP>(o, vp, part0 + 32 * j, s[j], lane);
+    }
+    if constexpr (WAVES == 2) {
+        __syncthreads();  // the planes are free: the second waves' results pass through them
+        floatx4* const pass = reinterpret_cast<floatx4*>(&planes[0][0]) + wave * (4 * NB + 1) * 64 + lane;
+        if (part0) {
+#pragma unroll
+            for (int i = 0; i < NB; ++i)
+#pragma unroll
+                for (int u = 0; u < 4; ++u) pass[(4 * i + u) * 64] = floatx4{o[i][4 * u], o[i][4 * u + 1], o[i][4 * u + 2], o[i][4 * u + 3]};
+            pass[4 * NB * 64] = floatx4{top, l, 0.f, 0.f};
+        }
+        __syncthreads();
+        if (part0) return;
+        const floatx4 other = pass[4 * NB * 64];
+        const float both = fmaxf(top, other[0]), base = both == -INFINITY ? 0.f : both;
+        const float mine = fast_exp2(top - base), theirs = fast_exp2(other[0] - base);
+        top = both;
+        l = l * mine + other[1] * theirs;
+#pragma unroll
+        for (int i = 0; i < NB; ++i)
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const floatx4 x = pass[(4 * i + u) * 64];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[i][4 * u + e] = o[i][4 * u + e] * mine + x[e] * theirs;
+            }
     }
     float unit = kDown2;
     if (any_not_finite(o)) {
@@ -341,7 +370,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void attn_split_kernel(Packe
     bool dst_vec = vec;
     if (tl.ranges > 1) {
         const int t = rho - tl.rho0;
-        const Partials part = partials(ws, a.n_kv, kv, gridDim.x / a.n_kv, w.item0 + w.range, kRowsPerWG, dim);
+        const Partials part = partials(ws, a.n_kv, kv, gridDim.x / a.n_kv, w.item0 + w.range, PER, dim);
         inv = 1.0f;
         dst = part.o + t * padded_dim(dim);
         dst_vec = true;
@@ -835,20 +864,23 @@ __global__ __launch_bounds__(256) void attn_split_dkv_join_kernel(PackedAttn a, 
 
 }  // namespace
 
-#define FMLH_BY_DIM(LAUNCH)                        \
-    do {                                           \
-        if (a.head_dim <= 32) LAUNCH(32);          \
-        else if (a.head_dim <= 64) LAUNCH(64);     \
-        else if (a.head_dim <= 96) LAUNCH(96);     \
-        else LAUNCH(128);                          \
-    } while (0)
-
-int attn_split_forward(const PackedAttn& a, uint32_t items, uint32_t budget, float* out, float* lse, const float* q, const float* k,
+int attn_split_forward(const PackedAttn& a, int per, uint32_t items, uint32_t budget, float* out, float* lse, const float* q, const float* k,
                        const float* v, float* ws, hipStream_t s) {
     const dim3 grid(items * a.n_kv);
-#define FMLH_LAUNCH(DP) hipLaunchKernelGGL((a.vec ? attn_split_kernel<DP, true> : attn_split_kernel<DP, false>), grid, dim3(256), 0, s, a, out, lse, q, k, v, ws, budget)
-    FMLH_BY_DIM(FMLH_LAUNCH);
+#define FMLH_LAUNCH_PER(DP, PER)                                                                                                \
+    hipLaunchKernelGGL((a.vec ? attn_split_kernel<DP, true, PER> : attn_split_kernel<DP, false, PER>), grid, dim3(256), 0, s, a, \
+                       out, lse, q, k, v, ws, budget)
+#define FMLH_LAUNCH(DP)                              \
+    do {                                             \
+        if (per == kRowsPerWG) FMLH_LAUNCH_PER(DP, kRowsPerWG); \
+        else FMLH_LAUNCH_PER(DP, kRowsPerWG / 2);    \
+    } while (0)
+    if (a.head_dim <= 32) FMLH_LAUNCH(32);
+    else if (a.head_dim <= 64) FMLH_LAUNCH(64);
+    else if (a.head_dim <= 96) FMLH_LAUNCH(96);
+    else FMLH_LAUNCH(128);
 #undef FMLH_LAUNCH
+#undef FMLH_LAUNCH_PER
     FMLH_LAUNCHED("attn_split_kernel");
     return FMLH_OK;
 }
