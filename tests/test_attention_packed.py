@@ -311,6 +311,34 @@ def test_values_and_gradients_at_the_ends_of_the_range(v, g, dim):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dim", [20, 64, 128])
+@pytest.mark.parametrize("v", [1.0, 1e30])
+@pytest.mark.parametrize("heads", [4, 96])
+def test_tiles_of_all_and_of_half_the_rows(heads, v, dim):
+    """Few tiles take half the rows each, many (96 heads) all of them; lengths at and around both."""
+    lens = [63, 64, 65, 1, 128, 129, 32, 97] if heads == 4 else [130, 66, 1]
+    c = Case(lens, lens, heads, heads // 2, dim, seed=21)
+    c.v = [(x * np.float32(v)).astype(np.float32) for x in c.v]
+    check(c)
+
+
+@pytest.mark.gpu
+def test_bad_keys_behind_a_row_in_the_same_tile():
+    """Half-row tiles whose second waves hold nothing but masked keys, some of them not finite."""
+    c = Case([40], [40], 2, 2, 32, seed=22)
+    clean = Case([40], [40], 2, 2, 32, seed=22)
+    c.k[0][33:] = np.nan
+    c.v[0][33:] = np.inf
+    c.build()
+    c.forward()
+    out, lse = c.read_rows(c.d_out.numpy()), c.d_lse.numpy()
+    for h in range(2):
+        r = reference(clean, 0, h)
+        close(out[0][:33, h], r["out"][:33], r["b_out"][:33], "out")
+        close(lse[h, :33], r["lse"][:33], r["b_lse"][:33], "lse")
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("klens", [[3000], [900, 2000]])
 def test_cut_keys_at_the_ends_of_the_range(klens):
     """The same where the keys are cut into ranges, on tiles of rows and on few rows."""
