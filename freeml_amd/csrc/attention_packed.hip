@@ -15,7 +15,7 @@
 // the order of work-groups.
 //
 // Here: a few rows over many keys, the joining of ranges of keys, plans and entry points.  Tiles of
-// 128 rows and the backward pass are in attention_packed_split.hip.
+// 64 and 128 rows and the backward pass are in attention_packed_split.hip.
 #include "attention_packed_device.h"
 
 #include <algorithm>
