@@ -448,6 +448,29 @@ def test_same_bits_every_time_and_on_other_workspaces():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("stride", [1 << 22, (1 << 22) + 4])
+def test_wide_row_strides(stride):
+    """Keys far apart, up to and beyond the stride that vector loads take: the bits of close ones."""
+    r, n, H, D = np.random.default_rng(31), 5, 2, 64
+    dev = fh.DeviceArray.from_host
+    off = dev(np.array([0, n], np.int32))
+    q = dev(r.standard_normal((n, H * D)).astype(np.float32))
+    kv = r.standard_normal((n, 2 * H * D)).astype(np.float32)
+    wide = np.zeros((n, stride), np.float32)
+    wide[:, :2 * H * D] = kv
+    results = []
+    for keys, rs in ((kv, 2 * H * D), (wide, stride)):
+        d_kv, out, lse = dev(keys), dev(np.zeros((n, H * D), np.float32)), dev(np.zeros((H, n), np.float32))
+        shape = fh.PackedAttention(n_seq=1, q_rows=n, k_rows=n, n_head=H, n_kv_head=1, head_dim=D, scale=0.125, q_off=off.ptr,
+                                   k_off=off.ptr, k_len=None, q_rs=H * D, o_rs=H * D, k_rs=rs, v_rs=rs, k_hs=D, v_hs=D)
+        assert fh.attention_packed_workspace(shape) == 0
+        fh.attention_packed(shape, out.ptr, lse.ptr, q.ptr, d_kv.ptr, d_kv.at(H * D))
+        results.append((out.numpy(), lse.numpy()))
+    assert np.all(results[0][0] == results[1][0]) and np.all(results[0][1] == results[1][1])
+    assert np.any(results[0][0] != 0)
+
+
+@pytest.mark.gpu
 def test_offsets_outside_the_rows_are_cut():
     """Offsets beyond the rows that exist, negative ones and lengths below zero read and write nothing outside."""
     c = Case([10, 20], [10, 20], 2, 1, 64, seed=1).build()
